@@ -8,6 +8,8 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
+from array import array
 from ctypes import POINTER, c_char_p, c_double, c_float, c_int, c_int64, c_size_t, c_uint32, c_void_p
 
 import torch
@@ -111,6 +113,15 @@ _PROTOTYPES: dict[str, tuple] = {
         [c_void_p, c_int, c_int64, c_void_p, c_int, c_int64, c_void_p, c_int64, c_void_p, c_int64]
         + [c_int, c_int, c_int, c_float, c_float, c_void_p],
     ),
+    "eo_adamw_scratch_bytes": (c_size_t, [c_int]),
+    "eo_adamw_step": (c_int, [c_int, c_void_p, c_char_p, c_void_p]),
+    "eo_grad_norm_scratch_bytes": (c_size_t, [c_int]),
+    "eo_grad_norm": (c_int, [c_int, c_void_p, c_float, c_int, c_void_p, c_void_p, c_size_t, c_void_p]),
+    "eo_quantize_blockwise": (
+        c_int,
+        [c_void_p, c_int, c_int64, c_int, c_int, c_uint32, c_void_p, c_void_p, c_void_p],
+    ),
+    "eo_dequantize_blockwise": (c_int, [c_void_p, c_void_p, c_int64, c_int, c_void_p, c_int, c_void_p]),
     "eo_peek_device_status_async": (c_int, [c_void_p, c_void_p]),
     "eo_debug_pair_schedule": (c_int, [c_int, c_int, c_int, c_int, c_int, c_int, c_void_p, c_int64, POINTER(c_int64)]),
     "eo_tp_gram_mirror": (c_int, [c_void_p, c_int, c_int64, c_void_p]),
@@ -753,3 +764,90 @@ def peek_device_status_async(pinned: torch.Tensor, device: torch.device) -> None
     with torch.cuda.device(device):
         rc = lib().eo_peek_device_status_async(pinned.data_ptr(), torch.cuda.current_stream(device).cuda_stream)
     _check(rc, "eo_peek_device_status_async")
+
+
+# ---- operators over lists of tensors ----------------------------------------------------------------------------------
+
+#: Tensors one launch takes, and elements that share an exponent byte of an 8-bit state.
+MAX_TENSORS_PER_LAUNCH = 384
+QUANT_BLOCK = 256
+
+KIND_PARAM_BF16, KIND_GRAD_BF16, KIND_REMAINDER = 1, 2, 4
+_DECAY_METHODS = {"decoupled": 0, "independent": 1, "palm": 2, "l2": 3}
+_CONFIG = struct.Struct("<dddddqQQQQiiII")  # eo_adamw_config
+
+
+def _launch(device: int, call, *args) -> int:
+    """``call(*args, stream)`` with ``device`` current, on its current stream."""
+    if torch.cuda.current_device() == device:
+        return call(*args, torch.cuda.current_stream(device).cuda_stream)
+    with torch.cuda.device(device):
+        return call(*args, torch.cuda.current_stream(device).cuda_stream)
+
+
+def adamw_step(
+    device: int, columns: list[list[int]], *, lr: float, betas: tuple[float, float], eps: float, weight_decay: float,
+    method: str, step: int, state_bits: int, seed: int = 0, first_index: int = 0, lr_tensor: torch.Tensor | None = None,
+    grad_scale: torch.Tensor | None = None,
+) -> None:  # fmt: skip
+    """One AdamW step; ``columns`` are the ten rows of ``eo_adamw_step``'s table, one integer per tensor."""
+    global launch_count
+    n = len(columns[0])
+    table = array("q")
+    for column in columns:
+        table.extend(column)
+    scratch, scratch_ptr, nbytes, on_device = None, 0, 0, lr_tensor is not None or any(columns[7])
+    if on_device:
+        nbytes = lib().eo_adamw_scratch_bytes(n)
+        scratch = torch.empty(nbytes, dtype=torch.uint8, device=f"cuda:{device}")
+        scratch_ptr = scratch.data_ptr()
+    config = _CONFIG.pack(
+        lr, betas[0], betas[1], eps, weight_decay, step,
+        lr_tensor.data_ptr() if lr_tensor is not None else 0, grad_scale.data_ptr() if grad_scale is not None else 0,
+        scratch_ptr, nbytes, _DECAY_METHODS[method], state_bits, seed, first_index,
+    )  # fmt: skip
+    launch_count += len(set(columns[9])) * -(-n // MAX_TENSORS_PER_LAUNCH) * (2 if on_device else 1)
+    rc = _launch(device, lib().eo_adamw_step, n, table.buffer_info()[0], config)
+    _check(rc, "eo_adamw_step")
+
+
+def grad_norm(device: int, columns: list[list[int]], max_norm: float, in_place: bool) -> torch.Tensor:
+    """Norm and clipping coefficient (fp32, shape (2,)) of the tensors of ``columns`` (addresses, element counts,
+    1 for bf16); ``in_place`` also multiplies them by the coefficient.  See ``eo_grad_norm``."""
+    global launch_count
+    n = len(columns[0])
+    table = array("q")
+    for column in columns:
+        table.extend(column)
+    out = torch.empty(2, dtype=torch.float32, device=f"cuda:{device}")
+    nbytes = lib().eo_grad_norm_scratch_bytes(n)
+    scratch = torch.empty(nbytes, dtype=torch.uint8, device=out.device)
+    launch_count += 1 + len(set(columns[2])) * -(-n // MAX_TENSORS_PER_LAUNCH) * (2 if in_place else 1)
+    rc = _launch(
+        device, lib().eo_grad_norm, n, table.buffer_info()[0], max_norm, 1 if in_place else 0, out.data_ptr(),
+        scratch.data_ptr(), nbytes,
+    )  # fmt: skip
+    _check(rc, "eo_grad_norm")
+    return out
+
+
+def quantize_blockwise(x: torch.Tensor, signed: bool, seed: int | None, codes: torch.Tensor, exponents: torch.Tensor) -> None:
+    """Codes and exponent bytes of the flat dense tensor ``x``; see ``eo_quantize_blockwise``."""
+    global launch_count
+    launch_count += 1
+    rc = _launch(
+        x.get_device(), lib().eo_quantize_blockwise, x.data_ptr(), 1 if x.dtype == torch.bfloat16 else 0, x.numel(),
+        1 if signed else 0, 0 if seed is None else 1, 0 if seed is None else seed, codes.data_ptr(), exponents.data_ptr(),
+    )  # fmt: skip
+    _check(rc, "eo_quantize_blockwise")
+
+
+def dequantize_blockwise(codes: torch.Tensor, exponents: torch.Tensor, signed: bool, out: torch.Tensor) -> None:
+    """The values that ``codes`` stand for, into the flat dense tensor ``out``; see ``eo_dequantize_blockwise``."""
+    global launch_count
+    launch_count += 1
+    rc = _launch(
+        codes.get_device(), lib().eo_dequantize_blockwise, codes.data_ptr(), exponents.data_ptr(), codes.numel(),
+        1 if signed else 0, out.data_ptr(), 1 if out.dtype == torch.bfloat16 else 0,
+    )  # fmt: skip
+    _check(rc, "eo_dequantize_blockwise")

@@ -17,6 +17,7 @@
 #include "gemm_sm100.cuh"
 #include "gemm_pair_sm100.cuh"
 #include "ns_small_sm100.cuh"
+#include "optimizer_step.cuh"
 
 namespace {
 
@@ -478,6 +479,84 @@ int launch_gemm(const void* A, int a_mn, int64_t lda, int64_t strideA, int64_t p
 
 }  // namespace
 
+// Helpers of the operators over lists of tensors (optimizer_step.cuh).
+
+namespace {
+inline bool aligned_to(const void* p, uintptr_t bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
+inline uintptr_t run_alignment(int dtype) { return dtype == EO_F32 ? 32 : 16; }  // of the wide accesses to eight elements
+inline bool known_dtype(int dtype) { return dtype == EO_F32 || dtype == EO_BF16; }
+
+// Chunks of the tensors in `table`: as many trips per CTA as leave every SM a few rounds of CTAs.  Less than
+// 2 kOptChunks + n of them.
+constexpr int64_t kOptChunks = 148 * 32;
+template <typename Table>
+int64_t cut_chunks(Table& table) {
+  long long total = 0;
+  for (int i = 0; i < table.n; ++i) total += table.t[i].numel;
+  long long trips = total / (eo::kOptTrip * kOptChunks);
+  table.trips = static_cast<int>(trips < 1 ? 1 : trips > (1 << 24) ? (1 << 24) : trips);
+  const long long chunk = static_cast<long long>(table.trips) * eo::kOptTrip;
+  int64_t chunks = 0;
+  for (int i = 0; i < table.n; ++i) {
+    table.first[i] = static_cast<uint32_t>(chunks);
+    chunks += (table.t[i].numel + chunk - 1) / chunk;
+  }
+  return chunks;
+}
+
+template <int kCapacity>
+int launch_adamw(eo::TensorTable<eo::AdamWEntry, kCapacity>& table, eo::AdamWScalars c, const eo_adamw_config& cfg, int kind,
+                 eo::AdamWFactors* factors, cudaStream_t s) {
+  const int64_t chunks = cut_chunks(table);
+  if (chunks > INT32_MAX) return fail(EO_ERR_BAD_ARG, "too many elements in one call");
+  const unsigned grid = static_cast<unsigned>(chunks);
+  if (factors != nullptr) {
+    eo::adamw_factors_kernel<kCapacity><<<1, 128, 0, s>>>(table, cfg.lr, cfg.dev_lr, cfg.beta1, cfg.beta2, cfg.weight_decay,
+                                                          cfg.decay_method, cfg.step, factors);
+    c.dev_factors = factors;
+  }
+#define EO_ADAMW(P, G, R)                                                                             \
+  do {                                                                                                \
+    if (cfg.state_bits == 8)                                                                          \
+      eo::adamw_kernel<P, G, R, true, kCapacity><<<grid, eo::kOptThreads, 0, s>>>(table, c);          \
+    else                                                                                              \
+      eo::adamw_kernel<P, G, R, false, kCapacity><<<grid, eo::kOptThreads, 0, s>>>(table, c);         \
+  } while (0)
+  switch (kind) {
+    case 0: EO_ADAMW(float, float, false); break;
+    case EO_KIND_GRAD_BF16: EO_ADAMW(float, __nv_bfloat16, false); break;
+    case EO_KIND_PARAM_BF16: EO_ADAMW(__nv_bfloat16, float, false); break;
+    case EO_KIND_PARAM_BF16 | EO_KIND_GRAD_BF16: EO_ADAMW(__nv_bfloat16, __nv_bfloat16, false); break;
+    case EO_KIND_PARAM_BF16 | EO_KIND_REMAINDER: EO_ADAMW(__nv_bfloat16, float, true); break;
+    default: EO_ADAMW(__nv_bfloat16, __nv_bfloat16, true); break;
+  }
+#undef EO_ADAMW
+  EO_CUDA(cudaGetLastError());
+  return EO_OK;
+}
+
+// Calls `launch(table)` with the non-empty tensors of [i0, i1) in a small or a large table.
+template <typename Entry, typename Fill, typename Launch>
+int over_tables(int n, Fill fill, Launch launch) {
+  int i = 0;
+  while (i < n) {
+    eo::TensorTable<Entry, eo::kOptLargeTable> big;
+    big.n = 0;
+    for (; i < n && big.n < eo::kOptLargeTable; ++i) big.n += fill(i, big.t[big.n]) ? 1 : 0;
+    if (big.n == 0) continue;
+    if (big.n <= eo::kOptSmallTable) {
+      eo::TensorTable<Entry, eo::kOptSmallTable> small;
+      small.n = big.n;
+      for (int k = 0; k < big.n; ++k) small.t[k] = big.t[k];
+      if (int rc = launch(small)) return rc;
+    } else if (int rc = launch(big)) {
+      return rc;
+    }
+  }
+  return EO_OK;
+}
+}  // namespace
+
 extern "C" {
 
 const char* eo_version(void) { return "eo_b200 0.1.0 sm_100a"; }
@@ -840,6 +919,190 @@ int eo_muon_apply_batch(int n, float* const* p, const void* const* update, int u
     else
       eo::muon_apply_mt_kernel<float><<<grid, eo::kEwThreads, 0, s>>>(t, shrink, extra_scale, lr);
   }
+  EO_CUDA(cudaGetLastError());
+  return EO_OK;
+}
+
+// ---- operators over lists of tensors (optimizer_step.cuh) ----
+
+size_t eo_adamw_scratch_bytes(int n) { return n > 0 ? static_cast<size_t>(n) * sizeof(eo::AdamWFactors) : 0; }
+
+int eo_adamw_step(int n, const int64_t* host_table, const eo_adamw_config* config, void* stream) {
+  DeviceInfo* dev = nullptr;
+  if (int rc = device_setup(&dev)) return rc;
+  if (n < 0 || (n > 0 && host_table == nullptr) || config == nullptr)
+    return fail(EO_ERR_BAD_ARG, "negative count or null pointer");
+  if (n == 0) return EO_OK;
+  const eo_adamw_config& cfg = *config;
+  if (cfg.state_bits != 8 && cfg.state_bits != 32) return fail(EO_ERR_BAD_ARG, "state_bits must be 8 or 32");
+  if (cfg.decay_method < 0 || cfg.decay_method > 3) return fail(EO_ERR_BAD_ARG, "unknown weight-decay method");
+  const int64_t *p = host_table, *g = p + n, *m = g + n, *v = m + n, *me = v + n, *ve = me + n, *r = ve + n, *step = r + n,
+                *numel = step + n, *kind = numel + n;
+  bool device_factors = cfg.dev_lr != nullptr;
+  unsigned kinds = 0;
+  for (int i = 0; i < n; ++i) {
+    if (numel[i] < 0) return fail(EO_ERR_BAD_ARG, "tensor %d: negative size", i);
+    if (numel[i] == 0) continue;
+    if (!p[i] || !g[i] || !m[i] || !v[i] || (cfg.state_bits == 8 && (!me[i] || !ve[i])))
+      return fail(EO_ERR_BAD_ARG, "tensor %d: null pointer", i);
+    if (kind[i] < 0 || kind[i] > 7 || ((kind[i] & EO_KIND_REMAINDER) && (!(kind[i] & EO_KIND_PARAM_BF16) || !r[i])))
+      return fail(EO_ERR_BAD_ARG, "tensor %d: unknown kind, or remainders without bf16 parameters", i);
+    if (step[i]) device_factors = true;
+    kinds |= 1u << kind[i];
+  }
+  if (cfg.step < 1 && !device_factors) return fail(EO_ERR_BAD_ARG, "step counts from 1");
+  if (device_factors && (cfg.scratch == nullptr || cfg.scratch_bytes < eo_adamw_scratch_bytes(n)))
+    return fail(EO_ERR_WORKSPACE, "adamw scratch: need %zu bytes, got %zu", eo_adamw_scratch_bytes(n), cfg.scratch_bytes);
+  eo::AdamWScalars c;
+  c.beta1 = static_cast<float>(cfg.beta1);
+  c.one_minus_beta1 = static_cast<float>(1.0 - cfg.beta1);
+  c.beta2 = static_cast<float>(cfg.beta2);
+  c.one_minus_beta2 = static_cast<float>(1.0 - cfg.beta2);
+  c.eps = static_cast<float>(cfg.eps);
+  c.l2 = cfg.decay_method == eo::kDecayL2 ? static_cast<float>(cfg.weight_decay) : 0.0f;
+  c.seed = cfg.seed;
+  c.f = eo::AdamWFactors{};
+  if (!device_factors)
+    c.f = eo::adamw_factors(cfg.lr, cfg.beta1, cfg.beta2, cfg.weight_decay, cfg.decay_method, cfg.step);
+  c.dev_factors = nullptr;
+  c.grad_scale = cfg.grad_scale;
+  eo::AdamWFactors* factors = device_factors ? static_cast<eo::AdamWFactors*>(cfg.scratch) : nullptr;
+  for (int k = 0; k < 8; ++k) {
+    if (!(kinds & (1u << k))) continue;
+    const uintptr_t ap = (k & EO_KIND_PARAM_BF16) ? 16 : 32, ag = (k & EO_KIND_GRAD_BF16) ? 16 : 32,
+                    as = cfg.state_bits == 8 ? 8 : 32;
+    auto fill = [&](int i, eo::AdamWEntry& t) {
+      if (numel[i] == 0 || kind[i] != k) return false;
+      t.p = reinterpret_cast<void*>(p[i]);
+      t.g = reinterpret_cast<const void*>(g[i]);
+      t.m = reinterpret_cast<void*>(m[i]);
+      t.v = reinterpret_cast<void*>(v[i]);
+      t.me = reinterpret_cast<uint8_t*>(me[i]);
+      t.ve = reinterpret_cast<uint8_t*>(ve[i]);
+      t.r = (k & EO_KIND_REMAINDER) ? reinterpret_cast<int16_t*>(r[i]) : nullptr;
+      t.step = reinterpret_cast<const long long*>(step[i]);
+      t.numel = numel[i];
+      t.index = cfg.first_index + static_cast<uint32_t>(i);
+      t.vec = aligned_to(t.p, ap) && aligned_to(t.g, ag) && aligned_to(t.m, as) && aligned_to(t.v, as) && aligned_to(t.r, 16);
+      return true;
+    };
+    auto launch = [&](auto& table) {
+      const int rc = launch_adamw(table, c, cfg, k, factors, static_cast<cudaStream_t>(stream));
+      if (factors != nullptr) factors += table.n;
+      return rc;
+    };
+    if (int rc = over_tables<eo::AdamWEntry>(n, fill, launch)) return rc;
+  }
+  return EO_OK;
+}
+
+size_t eo_grad_norm_scratch_bytes(int n) {
+  if (n < 0) return 0;
+  const size_t tables = static_cast<size_t>(n) / eo::kOptLargeTable + 2;  // two types
+  return sizeof(double) * (tables * 2 * kOptChunks + static_cast<size_t>(n));
+}
+
+int eo_grad_norm(int n, const int64_t* host_table, float max_norm, int in_place, float* out, void* scratch,
+                 size_t scratch_bytes, void* stream) {
+  DeviceInfo* dev = nullptr;
+  if (int rc = device_setup(&dev)) return rc;
+  if (n < 0 || (n > 0 && host_table == nullptr) || out == nullptr)
+    return fail(EO_ERR_BAD_ARG, "negative count or null pointer");
+  if (scratch == nullptr || scratch_bytes < eo_grad_norm_scratch_bytes(n))
+    return fail(EO_ERR_WORKSPACE, "grad norm scratch: need %zu bytes, got %zu", eo_grad_norm_scratch_bytes(n), scratch_bytes);
+  const int64_t *g = host_table, *numel = g + n, *dtype = numel + n;
+  unsigned types = 0;
+  for (int i = 0; i < n; ++i) {
+    if (numel[i] < 0 || (numel[i] > 0 && !g[i])) return fail(EO_ERR_BAD_ARG, "tensor %d: null pointer or negative size", i);
+    if (dtype[i] != EO_F32 && dtype[i] != EO_BF16) return fail(EO_ERR_BAD_ARG, "tensor %d: gradients are fp32 or bf16", i);
+    types |= 1u << dtype[i];
+  }
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  double* partials = static_cast<double*>(scratch);
+  int64_t used = 0;
+  for (int pass = 0; pass < (in_place ? 2 : 1); ++pass) {
+    for (int type = EO_F32; type <= EO_BF16; ++type) {
+      if (!(types & (1u << type))) continue;
+      auto fill = [&](int i, eo::GradEntry& t) {
+        if (numel[i] == 0 || dtype[i] != type) return false;
+        t.g = reinterpret_cast<void*>(g[i]);
+        t.numel = numel[i];
+        t.vec = aligned_to(t.g, run_alignment(type));
+        return true;
+      };
+      auto launch = [&](auto& table) -> int {
+        const int64_t chunks = cut_chunks(table);
+        constexpr int cap = sizeof(table.t) / sizeof(table.t[0]);
+        const unsigned grid = static_cast<unsigned>(chunks);
+        if (pass == 0) {
+          if (type == EO_F32)
+            eo::grad_sumsq_kernel<float, cap><<<grid, eo::kOptThreads, 0, s>>>(table, partials + used);
+          else
+            eo::grad_sumsq_kernel<__nv_bfloat16, cap><<<grid, eo::kOptThreads, 0, s>>>(table, partials + used);
+          used += chunks;
+        } else {
+          if (type == EO_F32)
+            eo::grad_scale_kernel<float, cap><<<grid, eo::kOptThreads, 0, s>>>(table, out + 1);
+          else
+            eo::grad_scale_kernel<__nv_bfloat16, cap><<<grid, eo::kOptThreads, 0, s>>>(table, out + 1);
+        }
+        return EO_OK;
+      };
+      if (int rc = over_tables<eo::GradEntry>(n, fill, launch)) return rc;
+    }
+    if (pass == 0) eo::grad_norm_final_kernel<<<1, eo::kEwThreads, 0, s>>>(partials, used, max_norm, out);
+  }
+  EO_CUDA(cudaGetLastError());
+  return EO_OK;
+}
+
+int eo_quantize_blockwise(const void* x, int dtype, int64_t numel, int is_signed, int random, uint32_t seed, uint8_t* codes,
+                          uint8_t* exponents, void* stream) {
+  DeviceInfo* dev = nullptr;
+  if (int rc = device_setup(&dev)) return rc;
+  if (!known_dtype(dtype)) return fail(EO_ERR_BAD_ARG, "values are fp32 or bf16");
+  if (numel < 0) return fail(EO_ERR_BAD_ARG, "negative size");
+  if (numel == 0) return EO_OK;
+  if (x == nullptr || codes == nullptr || exponents == nullptr) return fail(EO_ERR_BAD_ARG, "null pointer");
+  const int64_t grid = (numel + eo::kOptTrip - 1) / eo::kOptTrip;
+  if (grid > INT32_MAX) return fail(EO_ERR_BAD_ARG, "too many elements in one call");
+  const int vec = aligned_to(x, run_alignment(dtype)) && aligned_to(codes, 8);
+  const uint32_t key = eo::rounding_key(seed, 0, 0);
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const unsigned g = static_cast<unsigned>(grid);
+#define EO_QUANTIZE(T, S)                                                                                             \
+  eo::quantize_kernel<T, S><<<g, eo::kOptThreads, 0, s>>>(static_cast<const T*>(x), numel, vec, random, key, codes, exponents)
+  if (dtype == EO_F32) {
+    if (is_signed) EO_QUANTIZE(float, true); else EO_QUANTIZE(float, false);
+  } else {
+    if (is_signed) EO_QUANTIZE(__nv_bfloat16, true); else EO_QUANTIZE(__nv_bfloat16, false);
+  }
+#undef EO_QUANTIZE
+  EO_CUDA(cudaGetLastError());
+  return EO_OK;
+}
+
+int eo_dequantize_blockwise(const uint8_t* codes, const uint8_t* exponents, int64_t numel, int is_signed, void* out, int dtype,
+                            void* stream) {
+  DeviceInfo* dev = nullptr;
+  if (int rc = device_setup(&dev)) return rc;
+  if (!known_dtype(dtype)) return fail(EO_ERR_BAD_ARG, "values are fp32 or bf16");
+  if (numel < 0) return fail(EO_ERR_BAD_ARG, "negative size");
+  if (numel == 0) return EO_OK;
+  if (out == nullptr || codes == nullptr || exponents == nullptr) return fail(EO_ERR_BAD_ARG, "null pointer");
+  const int64_t grid = (numel + eo::kOptTrip - 1) / eo::kOptTrip;
+  if (grid > INT32_MAX) return fail(EO_ERR_BAD_ARG, "too many elements in one call");
+  const int vec = aligned_to(out, run_alignment(dtype)) && aligned_to(codes, 8);
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const unsigned g = static_cast<unsigned>(grid);
+#define EO_DEQUANTIZE(T, S) \
+  eo::dequantize_kernel<T, S><<<g, eo::kOptThreads, 0, s>>>(codes, exponents, numel, vec, static_cast<T*>(out))
+  if (dtype == EO_F32) {
+    if (is_signed) EO_DEQUANTIZE(float, true); else EO_DEQUANTIZE(float, false);
+  } else {
+    if (is_signed) EO_DEQUANTIZE(__nv_bfloat16, true); else EO_DEQUANTIZE(__nv_bfloat16, false);
+  }
+#undef EO_DEQUANTIZE
   EO_CUDA(cudaGetLastError());
   return EO_OK;
 }

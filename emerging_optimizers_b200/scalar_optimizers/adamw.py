@@ -1,0 +1,387 @@
+"""AdamW over many tensors at once, with moments in fp32 or in 8 bits.
+
+The scalar optimizer that a model's embeddings, output layer and 1-D parameters need beside the orthogonalized ones
+(the reference keeps its scalar optimizers in ``emerging_optimizers/scalar_optimizers``).  A step of a parameter group is
+one launch for each mix of types (up to 384 tensors), whatever their sizes.
+"""
+
+from __future__ import annotations
+
+from typing import Any, Callable, Sequence
+
+import torch
+import torch.optim as optim
+from torch.optim.optimizer import ParamsT
+
+from emerging_optimizers_b200 import _native, registry
+from emerging_optimizers_b200.mixin import WeightDecayT
+from emerging_optimizers_b200.scalar_optimizers.quantization import (
+    dequantize_blockwise,
+    exponent_count,
+    quantize_blockwise,
+)
+from emerging_optimizers_b200.utils import tensor_lists
+
+
+__all__ = ["AdamW", "adamw_step", "adamw_step_8bit"]
+
+_FLOATS = (torch.float32, torch.bfloat16)
+_F32, _U8, _I16, _I64 = (torch.float32,), (torch.uint8,), (torch.int16,), (torch.int64,)
+_MASK32 = (1 << 32) - 1
+
+
+def _check_hyperparameters(lr: Any, betas: Any, eps: float, weight_decay: float, method: str) -> None:
+    if not torch.is_tensor(lr) and not lr >= 0.0:
+        raise ValueError(f"Invalid learning rate: {lr}")
+    if not (len(betas) == 2 and all(0.0 <= b < 1.0 for b in betas)):
+        raise ValueError(f"Invalid betas: {betas}")
+    if not eps >= 0.0:
+        raise ValueError(f"Invalid epsilon: {eps}")
+    if not weight_decay >= 0.0:
+        raise ValueError(f"Invalid weight decay: {weight_decay}")
+    if method not in _native._DECAY_METHODS:
+        raise ValueError(f"Invalid weight decay method: {method}")
+
+
+def _device_scalar(value: Any, name: str, device: int, dtype: torch.dtype) -> torch.Tensor:
+    if not torch.is_tensor(value) or value.dtype != dtype or value.numel() != 1 or value.get_device() != device:
+        raise TypeError(f"{name} must be a {dtype} tensor of one element on cuda:{device}")
+    return value
+
+
+def _step(
+    params, grads, m, v, m_exponents, v_exponents, remainders, *, state_bits, lr, betas, eps, weight_decay, step,
+    weight_decay_method, grad_scale, seed=0, first_index=0,
+) -> None:  # fmt: skip
+    _check_hyperparameters(lr, betas, eps, weight_decay, weight_decay_method)
+    params = list(params)
+    n = len(params)
+    if n == 0:
+        return
+    device = tensor_lists.common_device(params, "params")
+    column = tensor_lists.addresses
+    p_ptrs = column(params, "params", device, _FLOATS)
+    numels = list(map(torch.Tensor.numel, params))
+    columns = [p_ptrs, column(grads, "grads", device, _FLOATS, numels)]
+    zeros = [0] * n
+    if state_bits == 8:
+        counts = [exponent_count(k) for k in numels]
+        columns += [
+            column(m, "exp_avgs", device, _U8, numels),
+            column(v, "exp_avg_sqs", device, _U8, numels),
+            column(m_exponents, "exp_avg_exponents", device, _U8, counts),
+            column(v_exponents, "exp_avg_sq_exponents", device, _U8, counts),
+        ]
+    else:
+        columns += [column(m, "exp_avgs", device, _F32, numels), column(v, "exp_avg_sqs", device, _F32, numels), zeros, zeros]
+    kinds = [
+        (p.dtype is torch.bfloat16) + 2 * (g.dtype is torch.bfloat16) for p, g in zip(params, grads)
+    ]  # fmt: skip
+    if remainders is None:
+        columns.append(zeros)
+    else:
+        if any(not k & _native.KIND_PARAM_BF16 for k in kinds):
+            raise TypeError("remainders go with bf16 parameters only")
+        columns.append(column(remainders, "remainders", device, _I16, numels))
+        kinds = [k | _native.KIND_REMAINDER for k in kinds]
+    written = {"params": columns[0], "exp_avgs": columns[2], "exp_avg_sqs": columns[3]}
+    if state_bits == 8:
+        written |= {"exp_avg_exponents": columns[4], "exp_avg_sq_exponents": columns[5]}
+    if remainders is not None:
+        written["remainders"] = columns[6]
+    tensor_lists.require_distinct(numels, **written)
+
+    if isinstance(step, int):
+        if step < 1:
+            raise ValueError(f"step counts from 1, got {step}")
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("a step number given as an int would be frozen into the captured graph: pass an int64 device tensor")
+        columns.append(zeros)
+    else:
+        steps = [step] * n if torch.is_tensor(step) else list(step)
+        columns.append(column(steps, "step", device, _I64, [1] * n))
+        step = 0
+    columns += [numels, kinds]
+    lr_tensor = None
+    if torch.is_tensor(lr):
+        if lr.is_cuda:
+            lr_tensor, lr = _device_scalar(lr, "lr", device, torch.float32), 0.0
+        else:
+            lr = float(lr)
+    if grad_scale is not None:
+        _device_scalar(grad_scale, "grad_scale", device, torch.float32)
+    if not (0 <= seed <= _MASK32):
+        raise ValueError(f"seed must be in [0, 2^32), got {seed}")
+    _native.adamw_step(
+        device, columns, lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, method=weight_decay_method, step=step,
+        state_bits=state_bits, seed=seed, first_index=first_index, lr_tensor=lr_tensor, grad_scale=grad_scale,
+    )  # fmt: skip
+    tensor_lists.mark_written(params)
+
+
+@torch.no_grad()
+def adamw_step(
+    params: Sequence[torch.Tensor],
+    grads: Sequence[torch.Tensor],
+    exp_avgs: Sequence[torch.Tensor],
+    exp_avg_sqs: Sequence[torch.Tensor],
+    *,
+    lr: float | torch.Tensor,
+    betas: tuple[float, float] = (0.9, 0.95),
+    eps: float = 1e-8,
+    weight_decay: float = 0.01,
+    step: int | torch.Tensor | Sequence[torch.Tensor],
+    weight_decay_method: WeightDecayT = "decoupled",
+    grad_scale: torch.Tensor | None = None,
+    remainders: Sequence[torch.Tensor] | None = None,
+) -> None:
+    """One AdamW step of a list of tensors, in place.
+
+    All arithmetic is fp32 with one rounding per operation, the moments are fp32.  Tensors are contiguous CUDA tensors
+    of one device; parameters and gradients fp32 or bf16 in any mix.
+
+    Args:
+        params, grads, exp_avgs, exp_avg_sqs: parameters, gradients, first and second moments, one of each per tensor.
+        lr, betas, eps, weight_decay: as usual; ``lr`` may be an fp32 device scalar.
+        step: number of this step, from 1; or int64 device scalars (one for all or one per tensor) holding it, which a
+            captured graph reads anew at every replay.
+        weight_decay_method: one of :data:`emerging_optimizers_b200.mixin.WeightDecayT`.
+        grad_scale: fp32 device scalar that multiplies every gradient as it is read (a clipping coefficient).
+        remainders: int16, one per tensor, for bf16 parameters: the low halves of their fp32 masters, master bits =
+            (bf16 bits << 16) + remainder.  Start with zeros.  Without them a bf16 parameter is rounded to nearest every
+            step and loses updates below half its last place.
+    """
+    _step(
+        params, grads, exp_avgs, exp_avg_sqs, None, None, remainders, state_bits=32, lr=lr, betas=betas, eps=eps,
+        weight_decay=weight_decay, step=step, weight_decay_method=weight_decay_method, grad_scale=grad_scale,
+    )  # fmt: skip
+
+
+@torch.no_grad()
+def adamw_step_8bit(
+    params: Sequence[torch.Tensor],
+    grads: Sequence[torch.Tensor],
+    exp_avgs: Sequence[torch.Tensor],
+    exp_avg_exponents: Sequence[torch.Tensor],
+    exp_avg_sqs: Sequence[torch.Tensor],
+    exp_avg_sq_exponents: Sequence[torch.Tensor],
+    *,
+    lr: float | torch.Tensor,
+    betas: tuple[float, float] = (0.9, 0.95),
+    eps: float = 1e-8,
+    weight_decay: float = 0.01,
+    step: int | torch.Tensor | Sequence[torch.Tensor],
+    seed: int,
+    weight_decay_method: WeightDecayT = "decoupled",
+    grad_scale: torch.Tensor | None = None,
+    remainders: Sequence[torch.Tensor] | None = None,
+) -> None:
+    """:func:`adamw_step` with moments in 8 bits (see :func:`quantize_blockwise`: first moments signed, second ones
+    unsigned; codes of the tensor's size and one exponent byte per 256 elements, zeros at the start).
+
+    The update uses the new moments before they are rounded.  They are then rounded at random, up with the probability
+    of the part cut off, by bits from ``seed``, the tensor's place in the list, the step number and the element: to
+    nearest, a moving average in 8 bits stands still as soon as a step moves it by less than half a unit.
+    """
+    _step(
+        params, grads, exp_avgs, exp_avg_sqs, exp_avg_exponents, exp_avg_sq_exponents, remainders, state_bits=8, lr=lr,
+        betas=betas, eps=eps, weight_decay=weight_decay, step=step, weight_decay_method=weight_decay_method,
+        grad_scale=grad_scale, seed=seed,
+    )  # fmt: skip
+
+
+def _memory_order(t: torch.Tensor) -> tuple[int, ...] | None:
+    """Order of the dimensions of a dense tensor from the slowest to the fastest; None for a contiguous one."""
+    if t.is_contiguous():
+        return None
+    order = tuple(sorted(range(t.dim()), key=lambda d: (-t.stride(d), -t.size(d))))
+    if not t.permute(order).is_contiguous():
+        raise ValueError(f"AdamW needs dense parameters, got shape {tuple(t.shape)} with strides {t.stride()}")
+    return order
+
+
+def _flat(t: torch.Tensor, order: tuple[int, ...] | None) -> torch.Tensor:
+    """``t`` seen in memory order, a copy only if it is laid out otherwise."""
+    t = t.detach()
+    return (t if order is None else t.permute(order)).contiguous()
+
+
+@registry.register_optimizer("adamw")
+class AdamW(optim.Optimizer):
+    """AdamW whose step takes all tensors of a group in one launch.
+
+    Parameters are fp32 or bf16 and dense, on CUDA; gradients fp32 or bf16.  See :func:`adamw_step` for the arithmetic.
+
+    Args:
+        params: parameters or parameter groups (groups may set ``lr``, ``betas``, ``eps`` and ``weight_decay``).
+        lr: learning rate; an fp32 device scalar is read anew at every replay of a captured step.
+        betas, eps, weight_decay: as usual.
+        weight_decay_method: one of :data:`emerging_optimizers_b200.mixin.WeightDecayT`.
+        state_bits: 32, or 8 for moments of one byte each (2 bytes a parameter in place of 8; see
+            :func:`adamw_step_8bit`).
+        master_remainder: keep for bf16 parameters the low 16 bits of an fp32 master in ``state["remainder"]``.
+        capturable: count steps in device memory, so that :meth:`step` can be captured into a CUDA graph.  Run a step
+            before the capture: it creates the state.
+        seed: seed of the random rounding of 8-bit moments.
+    """
+
+    def __init__(
+        self,
+        params: ParamsT,
+        lr: float | torch.Tensor = 3e-4,
+        betas: tuple[float, float] = (0.9, 0.95),
+        eps: float = 1e-8,
+        weight_decay: float = 0.01,
+        *,
+        weight_decay_method: WeightDecayT = "decoupled",
+        state_bits: int = 32,
+        master_remainder: bool = False,
+        capturable: bool = False,
+        seed: int = 0,
+    ) -> None:
+        _check_hyperparameters(lr, betas, eps, weight_decay, weight_decay_method)
+        if not 0 <= seed <= _MASK32:
+            raise ValueError(f"seed must be in [0, 2^32), got {seed}")
+        if state_bits not in (8, 32):
+            raise ValueError(f"state_bits must be 8 or 32, got {state_bits}")
+        self.weight_decay_method = weight_decay_method
+        self.state_bits = state_bits
+        self.master_remainder = master_remainder
+        self.capturable = capturable
+        self.seed = seed
+        super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay))
+
+    # -- state -------------------------------------------------------------------------------------------------------
+
+    def _has_remainder(self, p: torch.Tensor) -> bool:
+        return self.master_remainder and p.dtype == torch.bfloat16
+
+    def _new_state(self, p: torch.Tensor) -> dict:
+        if p.dtype not in _FLOATS:
+            raise TypeError(f"AdamW takes torch.float32 or torch.bfloat16 parameters, got {p.dtype}")
+        _native.require_cuda(p, "a parameter of AdamW")
+        _memory_order(p)
+        state: dict = {"step": torch.zeros((), dtype=torch.int64, device=p.device) if self.capturable else 0}
+        dtype = torch.uint8 if self.state_bits == 8 else torch.float32
+        for name in ("exp_avg", "exp_avg_sq"):
+            state[name] = torch.zeros_like(p, dtype=dtype, memory_format=torch.preserve_format)
+            if self.state_bits == 8:
+                state[f"{name}_exponents"] = torch.zeros(exponent_count(p.numel()), dtype=torch.uint8, device=p.device)
+        if self._has_remainder(p):
+            state["remainder"] = torch.zeros_like(p, dtype=torch.int16, memory_format=torch.preserve_format)
+        return state
+
+    def moments(self, p: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+        """First and second moment of ``p`` as new fp32 tensors, whatever they are stored in."""
+        state = self.state[p]
+        return tuple(self._values(state, name, signed) for name, signed in (("exp_avg", True), ("exp_avg_sq", False)))  # type: ignore[return-value]
+
+    @staticmethod
+    def _values(state: dict, name: str, signed: bool) -> torch.Tensor:
+        x = state[name]
+        if x.dtype != torch.uint8:
+            return x.clone()
+        order = _memory_order(x)
+        values = dequantize_blockwise(_flat(x, order), state[f"{name}_exponents"], signed=signed)
+        return values if order is None else values.permute([order.index(d) for d in range(x.dim())])
+
+    # -- step --------------------------------------------------------------------------------------------------------
+
+    @torch.no_grad()
+    def step(  # type: ignore[override]
+        self, closure: Callable[[], float] | None = None, *, grad_scale: torch.Tensor | None = None
+    ) -> None:
+        """One step.  ``grad_scale`` (an fp32 device scalar, for instance the coefficient of
+        :func:`emerging_optimizers_b200.utils.clip_coefficient`) multiplies the gradients as they are read."""
+        if closure is not None:
+            raise ValueError("closure is not supported")
+        first_index = 0
+        for group in self.param_groups:
+            # one call per device and step number; with device counters one per device
+            calls: dict[tuple, list[torch.Tensor]] = {}
+            for p in group["params"]:
+                grad = p.grad
+                if grad is None:
+                    continue
+                if grad.is_sparse:
+                    raise RuntimeError("AdamW does not support sparse gradients")
+                state = self.state[p]
+                if not state:
+                    if p.is_cuda and torch.cuda.is_current_stream_capturing():
+                        raise RuntimeError("run a step before capturing one: the state must exist when the capture begins")
+                    state.update(self._new_state(p))
+                step = 0 if self.capturable else state["step"] + 1
+                calls.setdefault((p.get_device(), step, self._has_remainder(p)), []).append(p)
+            for (_, step, remainder), params in calls.items():
+                self._call(group, params, step, remainder, grad_scale, first_index)
+                first_index += len(params)
+        return None
+
+    def _call(self, group, params, step, remainder, grad_scale, first_index) -> None:  # type: ignore[no-untyped-def]
+        states = [self.state[p] for p in params]
+        orders = [None if p.is_contiguous() else _memory_order(p) for p in params]
+        plain = not any(orders)
+
+        def column(name):  # type: ignore[no-untyped-def]
+            ts = [s[name] for s in states]
+            return ts if plain else [_flat(t, o) for t, o in zip(ts, orders)]
+
+        grads = [p.grad for p in params]
+        grads = [g if o is None and g.is_contiguous() else _flat(g, o) for g, o in zip(grads, orders)]
+        if self.capturable:
+            step = [s["step"] for s in states]
+            torch._foreach_add_(step, 1)
+        exponents = [[s[name] for s in states] for name in ("exp_avg_exponents", "exp_avg_sq_exponents")] if self.state_bits == 8 else (None, None)
+        _step(
+            params if plain else [_flat(p, o) for p, o in zip(params, orders)], grads, column("exp_avg"), column("exp_avg_sq"),
+            *exponents, column("remainder") if remainder else None, state_bits=self.state_bits, lr=group["lr"],
+            betas=group["betas"], eps=group["eps"], weight_decay=group["weight_decay"], step=step,
+            weight_decay_method=self.weight_decay_method, grad_scale=grad_scale, seed=self.seed, first_index=first_index,
+        )  # fmt: skip
+        if not self.capturable:
+            for s in states:
+                s["step"] = step
+
+    # -- checkpoints -------------------------------------------------------------------------------------------------
+
+    def load_state_dict(self, state_dict: dict[str, Any]) -> None:
+        """Load a state that this class or ``torch.optim.AdamW`` wrote.
+
+        Moments of the other width are converted (32 to 8 bits: rounded to nearest); types are kept as this optimizer
+        has them, whatever the parameter's.
+        """
+        saved = state_dict["state"]
+        super().load_state_dict({**state_dict, "state": {}})
+        ids = [i for group in state_dict["param_groups"] for i in group["params"]]
+        params = [p for group in self.param_groups for p in group["params"]]
+        for i, p in zip(ids, params):
+            if i in saved and saved[i]:
+                self.state[p] = self._loaded_state(p, saved[i])
+
+    @torch.no_grad()
+    def _loaded_state(self, p: torch.Tensor, saved: dict) -> dict:
+        state = self._new_state(p)
+        if self.capturable:
+            state["step"].fill_(int(saved["step"]))
+        else:
+            state["step"] = int(saved["step"])
+        for name, signed in (("exp_avg", True), ("exp_avg_sq", False)):
+            x = saved[name].to(p.device)
+            if x.shape != p.shape:
+                raise ValueError(f"{name} of shape {tuple(x.shape)} does not fit a parameter of shape {tuple(p.shape)}")
+            exponents = f"{name}_exponents"
+            if x.dtype == torch.uint8 and self.state_bits == 8 and x.stride() == p.stride():
+                state[name].copy_(x)
+                state[exponents].copy_(saved[exponents])
+                continue
+            if x.dtype == torch.uint8:
+                x = self._values({name: x, exponents: saved[exponents].to(p.device)}, name, signed)
+            if self.state_bits == 8:
+                order = _memory_order(p)
+                codes, state[exponents] = quantize_blockwise(_flat(torch.empty_like(p, dtype=torch.float32).copy_(x), order), signed=signed)
+                _flat(state[name], order).copy_(codes)
+            else:
+                state[name].copy_(x)
+        if "remainder" in state and "remainder" in saved:
+            state["remainder"].copy_(saved["remainder"])
+        return state

@@ -1,6 +1,6 @@
-"""Precision switch and process-group helpers used by the orthogonalization path.
+"""Precision switch and process-group helpers used by the orthogonalization path, and gradient clipping.
 
-Same public names and behaviour as ``emerging_optimizers/utils/__init__.py:25-54`` of the reference.
+The former have the public names and behaviour of ``emerging_optimizers/utils/__init__.py:25-54`` of the reference.
 """
 
 from __future__ import annotations
@@ -9,8 +9,19 @@ from typing import Literal
 
 import torch
 
+from emerging_optimizers_b200.utils.grad_norm import clip_coefficient, clip_grad_norm_, clip_grads_, global_grad_norm
 
-__all__ = ["fp32_matmul_precision", "FP32MatmulPrecT", "get_pg_size", "get_pg_rank"]
+
+__all__ = [
+    "FP32MatmulPrecT",
+    "clip_coefficient",
+    "clip_grad_norm_",
+    "clip_grads_",
+    "fp32_matmul_precision",
+    "get_pg_rank",
+    "get_pg_size",
+    "global_grad_norm",
+]
 
 FP32MatmulPrecT = Literal["highest", "high", "medium"]
 

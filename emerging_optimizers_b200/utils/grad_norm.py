@@ -1,0 +1,79 @@
+"""Global gradient norm and clipping over many tensors in a few launches, without a synchronisation.
+
+The clipping coefficient stays on the device: :func:`clip_coefficient` hands it to
+``AdamW.step(grad_scale=...)``, which then scales the gradients as it reads them, so that they are read once for the
+norm and never written back.  :func:`clip_grads_` / :func:`clip_grad_norm_` scale them in place for every other consumer.
+"""
+
+from __future__ import annotations
+
+import math
+from typing import Iterable, Sequence
+
+import torch
+
+from emerging_optimizers_b200 import _native
+from emerging_optimizers_b200.utils import tensor_lists
+
+
+__all__ = ["clip_coefficient", "clip_grad_norm_", "clip_grads_", "global_grad_norm"]
+
+_DTYPES = (torch.float32, torch.bfloat16)
+
+
+def _norm(grads: Sequence[torch.Tensor], max_norm: float, in_place: bool) -> torch.Tensor:
+    grads = list(grads)
+    if not grads:
+        raise ValueError("no gradients given")
+    if not max_norm >= 0.0:
+        raise ValueError(f"max_norm must not be negative, got {max_norm}")
+    device = tensor_lists.common_device(grads, "grads")
+    ptrs = tensor_lists.addresses(grads, "grads", device, _DTYPES)
+    numels = list(map(torch.Tensor.numel, grads))
+    if in_place:
+        tensor_lists.require_distinct(numels, grads=ptrs)
+    out = _native.grad_norm(device, [ptrs, numels, [g.dtype is torch.bfloat16 for g in grads]], max_norm, in_place)
+    if in_place:
+        tensor_lists.mark_written(grads)
+    return out
+
+
+@torch.no_grad()
+def global_grad_norm(grads: Sequence[torch.Tensor]) -> torch.Tensor:
+    """2-norm of all elements of ``grads`` (contiguous fp32 or bf16 CUDA tensors of one device) as an fp32 scalar
+    tensor.  Squares are summed in float64 in a fixed order: the same call gives the same bits."""
+    return _norm(grads, math.inf, False)[0]
+
+
+@torch.no_grad()
+def clip_coefficient(grads: Sequence[torch.Tensor], max_norm: float) -> tuple[torch.Tensor, torch.Tensor]:
+    """``(norm, min(1, max_norm / (norm + 1e-6)))`` as fp32 scalar tensors on the device; the gradients stay as they are.
+
+    Pass the coefficient to ``AdamW.step(grad_scale=...)``.  A norm that is NaN gives a coefficient that is NaN.
+    """
+    out = _norm(grads, max_norm, False)
+    return out[0], out[1]
+
+
+@torch.no_grad()
+def clip_grads_(grads: Sequence[torch.Tensor], max_norm: float) -> torch.Tensor:
+    """Multiply all of ``grads`` in place by ``min(1, max_norm / (norm + 1e-6))``; returns the norm from before."""
+    return _norm(grads, max_norm, True)[0]
+
+
+def clip_grad_norm_(
+    parameters: torch.Tensor | Iterable[torch.Tensor], max_norm: float, *, error_if_nonfinite: bool = False
+) -> torch.Tensor:
+    """Clip the global 2-norm of the gradients of ``parameters`` in place, as ``torch.nn.utils.clip_grad_norm_`` does.
+
+    Parameters without a gradient are passed over; with none left the result is 0.  ``error_if_nonfinite`` raises
+    ``RuntimeError`` before anything is scaled if the norm is infinite or NaN (and waits for the device to know).
+    """
+    if isinstance(parameters, torch.Tensor):
+        parameters = [parameters]
+    grads = [p.grad for p in parameters if p.grad is not None]
+    if not grads:
+        return torch.tensor(0.0)
+    if error_if_nonfinite and not math.isfinite(float(global_grad_norm(grads))):
+        raise RuntimeError("the total norm of the gradients is not finite, so they cannot be clipped")
+    return clip_grads_(grads, max_norm)

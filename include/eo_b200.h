@@ -385,6 +385,74 @@ int eo_gemm_multicast(const void* A, int a_mn_major, int64_t lda, const void* B,
  */
 int eo_peek_device_status_async(uint32_t* pinned_host_code, void* stream);
 
+/* ---- Operators over lists of tensors --------------------------------------------------------------------------- */
+
+/* Element types of these operators. */
+enum { EO_F32 = 0, EO_BF16 = 1 };
+/* Kind of a tensor of an AdamW step: which of its parts are bf16, and whether it has remainders. */
+enum { EO_KIND_PARAM_BF16 = 1, EO_KIND_GRAD_BF16 = 2, EO_KIND_REMAINDER = 4 };
+
+/*
+ * AdamW step of `n` tensors.  All arithmetic is fp32, one rounding per operation:
+ *   g = grad * grad_scale (+ weight_decay * p with method 3), p = p * decay,
+ *   m = beta1 m + (1 - beta1) g,  v = beta2 v + (1 - beta2) g^2,
+ *   p = p - (m / (sqrt(v) / sqrt(1 - beta2^t) + eps)) * lr / (1 - beta1^t)
+ * with decay = 1 - lr weight_decay (method 0, "decoupled"), 1 - weight_decay (1, "independent"),
+ * 1 - lr^2 weight_decay (2, "palm") or 1 (3, "l2").
+ *
+ * host_table: ten rows of n int64 each: addresses of the parameters, gradients, first moments, second moments,
+ * exponent bytes of the first and of the second moments (8-bit states, else 0), remainders (or 0), device step counters
+ * (int64, or 0), then the element counts and the kinds (EO_KIND_* flags; 0: fp32 parameters and gradients).  Tensors are
+ * flat and dense, any alignment of their element type; the wide accesses are used where p, g, m, v and remainders are
+ * aligned for eight elements (fp32: 32 bytes, 16-bit types: 16, codes: 8).  Empty tensors are skipped.
+ *
+ * state_bits 32: m, v fp32.  state_bits 8: m, v are codes of one byte per element with one exponent byte per 256
+ * elements (see eo_quantize_blockwise), rounded at random with bits from (seed, first_index + place in the list, step,
+ * element).  Remainders (int16, bf16 parameters only): the fp32 master of a parameter is (bf16 bits << 16) + remainder.
+ *
+ * `step` counts from 1.  With `dev_lr` or device step counters the factors that depend on them are computed by a small
+ * kernel into `scratch` (eo_adamw_scratch_bytes(n) bytes, 16-byte aligned), so that a captured step can be replayed;
+ * the counters are read, not advanced.  `grad_scale`: device fp32 scalar or NULL (1).
+ *
+ * Stands in for the scalar AdamW updates of emerging_optimizers/scalar_optimizers, one call for a list of parameters.
+ */
+typedef struct eo_adamw_config {
+  double lr, beta1, beta2, eps, weight_decay;
+  int64_t step;
+  const float* dev_lr;
+  const float* grad_scale;
+  void* scratch;
+  size_t scratch_bytes;
+  int32_t decay_method, state_bits;
+  uint32_t seed, first_index;
+} eo_adamw_config;
+size_t eo_adamw_scratch_bytes(int n);
+int eo_adamw_step(int n, const int64_t* host_table, const eo_adamw_config* config, void* stream);
+
+/*
+ * Global gradient norm of `n` flat dense tensors, fp32 and bf16 mixed as they come.  host_table: three rows of n int64
+ * (addresses, element counts, EO_F32 / EO_BF16).  Squares are summed in float64 in a fixed order.
+ * out[0] = norm, out[1] = min(1, max_norm / (norm + 1e-6)), fp32, in device memory; NaN stays NaN.
+ * in_place: the tensors are multiplied by out[1] afterwards (bf16 rounded to nearest even; untouched when it is 1).
+ * `scratch`: eo_grad_norm_scratch_bytes(n) bytes, 8-byte aligned.
+ */
+size_t eo_grad_norm_scratch_bytes(int n);
+int eo_grad_norm(int n, const int64_t* host_table, float max_norm, int in_place, float* out, void* scratch,
+                 size_t scratch_bytes, void* stream);
+
+/*
+ * 8-bit block-scaled numbers: codes (one byte per element) and one byte per block of 256 elements, the fp32 exponent
+ * field of the block's largest finite magnitude (at least 1).  is_signed: sign, 4 exponent and 3 mantissa bits, down to
+ * 2^-16 of the block's power of two; otherwise 5 exponent and 3 mantissa bits, down to 2^-32, where a value above zero never
+ * becomes zero.  Rounded to nearest (halves away from zero) or, with `random`, up with the probability of the part cut
+ * off, by bits from (seed, element).  What is not finite (unsigned: or is negative) reads back as NaN.  Values lie
+ * exactly in bf16 and fp32 as long as they are normal numbers there.
+ */
+int eo_quantize_blockwise(const void* x, int dtype, int64_t numel, int is_signed, int random, uint32_t seed, uint8_t* codes,
+                          uint8_t* exponents, void* stream);
+int eo_dequantize_blockwise(const uint8_t* codes, const uint8_t* exponents, int64_t numel, int is_signed, void* out, int dtype,
+                            void* stream);
+
 #ifdef __cplusplus
 }
 #endif
