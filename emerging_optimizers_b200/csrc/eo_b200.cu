@@ -515,12 +515,16 @@ int launch_adamw(eo::TensorTable<eo::AdamWEntry, kCapacity>& table, eo::AdamWSca
                                                           cfg.decay_method, cfg.step, factors);
     c.dev_factors = factors;
   }
-#define EO_ADAMW(P, G, R)                                                                             \
-  do {                                                                                                \
-    if (cfg.state_bits == 8)                                                                          \
-      eo::adamw_kernel<P, G, R, true, kCapacity><<<grid, eo::kOptThreads, 0, s>>>(table, c);          \
-    else                                                                                              \
-      eo::adamw_kernel<P, G, R, false, kCapacity><<<grid, eo::kOptThreads, 0, s>>>(table, c);         \
+#define EO_ADAMW(P, G, R)                                                                                  \
+  do {                                                                                                     \
+    if (cfg.state_bits == 8) {                                                                             \
+      const auto kernel = eo::adamw_kernel<P, G, R, true, kCapacity>;                                      \
+      constexpr int bytes = eo::AdamWRing<P, G, R>::kCtaBytes;                                             \
+      EO_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));           \
+      kernel<<<grid, eo::kOptThreads, bytes, s>>>(table, c);                                               \
+    } else {                                                                                               \
+      eo::adamw_kernel<P, G, R, false, kCapacity><<<grid, eo::kOptThreads, 0, s>>>(table, c);              \
+    }                                                                                                      \
   } while (0)
   switch (kind) {
     case 0: EO_ADAMW(float, float, false); break;
@@ -1064,7 +1068,7 @@ int eo_quantize_blockwise(const void* x, int dtype, int64_t numel, int is_signed
   if (numel < 0) return fail(EO_ERR_BAD_ARG, "negative size");
   if (numel == 0) return EO_OK;
   if (x == nullptr || codes == nullptr || exponents == nullptr) return fail(EO_ERR_BAD_ARG, "null pointer");
-  const int64_t grid = (numel + eo::kOptTrip - 1) / eo::kOptTrip;
+  const int64_t grid = (numel + eo::kQuantChunk - 1) / eo::kQuantChunk;
   if (grid > INT32_MAX) return fail(EO_ERR_BAD_ARG, "too many elements in one call");
   const int vec = aligned_to(x, run_alignment(dtype)) && aligned_to(codes, 8);
   const uint32_t key = eo::rounding_key(seed, 0, 0);
@@ -1090,7 +1094,7 @@ int eo_dequantize_blockwise(const uint8_t* codes, const uint8_t* exponents, int6
   if (numel < 0) return fail(EO_ERR_BAD_ARG, "negative size");
   if (numel == 0) return EO_OK;
   if (out == nullptr || codes == nullptr || exponents == nullptr) return fail(EO_ERR_BAD_ARG, "null pointer");
-  const int64_t grid = (numel + eo::kOptTrip - 1) / eo::kOptTrip;
+  const int64_t grid = (numel + eo::kQuantChunk - 1) / eo::kQuantChunk;
   if (grid > INT32_MAX) return fail(EO_ERR_BAD_ARG, "too many elements in one call");
   const int vec = aligned_to(out, run_alignment(dtype)) && aligned_to(codes, 8);
   cudaStream_t s = static_cast<cudaStream_t>(stream);

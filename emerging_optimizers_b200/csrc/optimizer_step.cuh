@@ -12,8 +12,11 @@
 #pragma once
 
 #include <cuda_bf16.h>
+#include <cuda_fp16.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
+
+#include <type_traits>
 
 namespace eo {
 
@@ -23,153 +26,166 @@ constexpr int kOptTrip = kOptThreads / 32 * kOptRun;          // elements a CTA 
 constexpr int kOptSmallTable = 24, kOptLargeTable = 384;      // tensors per launch
 
 // ---- memory access ---------------------------------------------------------------------------------------------------
+// A lane's eight elements of a run as they lie in memory.  get / put: elements 8 l .. 8 l + 7 from their own address (plus
+// kOffset elements, an immediate), one wide access; get_some / put_some: elements l, l + 32, ... of the run at `p`, guarded by
+// `left` (elements beyond the end read as zero and are not written).
 
-__device__ __forceinline__ void load_run(const float* p, float (&x)[8]) {
-  asm volatile("ld.global.L1::no_allocate.v8.f32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
-               : "=f"(x[0]), "=f"(x[1]), "=f"(x[2]), "=f"(x[3]), "=f"(x[4]), "=f"(x[5]), "=f"(x[6]), "=f"(x[7])
-               : "l"(p));
-}
-__device__ __forceinline__ void store_run(float* p, const float (&x)[8]) {
-  asm volatile("st.global.v8.f32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "f"(x[0]), "f"(x[1]), "f"(x[2]), "f"(x[3]),
-               "f"(x[4]), "f"(x[5]), "f"(x[6]), "f"(x[7])
-               : "memory");
-}
+template <int kBytes>
 __device__ __forceinline__ uint4 load_16(const void* p) {
   uint4 v;
-  asm volatile("ld.global.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+  asm volatile("ld.global.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4+%5];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "l"(p), "n"(kBytes));
   return v;
 }
+template <int kBytes>
 __device__ __forceinline__ uint2 load_8(const void* p) {
   uint2 v;
-  asm volatile("ld.global.L1::no_allocate.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p));
+  asm volatile("ld.global.L1::no_allocate.v2.u32 {%0,%1}, [%2+%3];" : "=r"(v.x), "=r"(v.y) : "l"(p), "n"(kBytes));
   return v;
 }
-__device__ __forceinline__ void store_16(void* p, uint4 v) { *reinterpret_cast<uint4*>(p) = v; }
-__device__ __forceinline__ void store_8(void* p, uint2 v) { *reinterpret_cast<uint2*>(p) = v; }
 
-__device__ __forceinline__ float bf16_bits_to_f32(uint32_t h) { return __uint_as_float(h << 16); }
-__device__ __forceinline__ uint32_t f32_to_bf16_bits(float x) { return __bfloat16_as_ushort(__float2bfloat16_rn(x)); }
-
-__device__ __forceinline__ void load_run(const __nv_bfloat16* p, float (&x)[8]) {
-  const uint4 v = load_16(p);
-  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-  for (int k = 0; k < 4; ++k) {
-    x[2 * k] = __uint_as_float(w[k] << 16);
-    x[2 * k + 1] = __uint_as_float(w[k] & 0xffff0000u);
-  }
-}
-__device__ __forceinline__ void store_run(__nv_bfloat16* p, const float (&x)[8]) {
-  uint32_t w[4];
-#pragma unroll
-  for (int k = 0; k < 4; ++k) {
-    const __nv_bfloat162 h = __floats2bfloat162_rn(x[2 * k], x[2 * k + 1]);
-    w[k] = *reinterpret_cast<const uint32_t*>(&h);
-  }
-  store_16(p, make_uint4(w[0], w[1], w[2], w[3]));
-}
-__device__ __forceinline__ float to_f32(float x) { return x; }
-__device__ __forceinline__ float to_f32(__nv_bfloat16 x) { return __bfloat162float(x); }
-__device__ __forceinline__ void from_f32(float* p, float x) { *p = x; }
-__device__ __forceinline__ void from_f32(__nv_bfloat16* p, float x) { *p = __float2bfloat16_rn(x); }
-
-// The run of `left` elements (from `x`) as eight values per lane; elements beyond the end read as zero.
 template <typename T>
-__device__ __forceinline__ void load_lane(const T* x, long long left, int lane, bool vec, float (&out)[8]) {
-  if (vec) {
-    load_run(x + 8 * lane, out);
-  } else {
-#pragma unroll
-    for (int k = 0; k < 8; ++k) out[k] = (32 * k + lane < left) ? to_f32(x[32 * k + lane]) : 0.0f;
+struct Run;
+
+template <>
+struct __align__(16) Run<float> {
+  float x[8];
+  template <int kOffset = 0>
+  __device__ __forceinline__ void get(const float* p) {
+    asm volatile("ld.global.L1::no_allocate.v8.f32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8+%9];"
+                 : "=f"(x[0]), "=f"(x[1]), "=f"(x[2]), "=f"(x[3]), "=f"(x[4]), "=f"(x[5]), "=f"(x[6]), "=f"(x[7])
+                 : "l"(p), "n"(4 * kOffset));
   }
-}
-template <typename T>
-__device__ __forceinline__ void store_lane(T* x, long long left, int lane, bool vec, const float (&v)[8]) {
-  if (vec) {
-    store_run(x + 8 * lane, v);
-  } else {
+  __device__ __forceinline__ void put(float* p) const {
+    asm volatile("st.global.v8.f32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "f"(x[0]), "f"(x[1]), "f"(x[2]), "f"(x[3]),
+                 "f"(x[4]), "f"(x[5]), "f"(x[6]), "f"(x[7])
+                 : "memory");
+  }
+  __device__ __forceinline__ void get_some(const float* p, long long left, int lane) {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) x[k] = (32 * k + lane < left) ? p[32 * k + lane] : 0.0f;
+  }
+  __device__ __forceinline__ void put_some(float* p, long long left, int lane) const {
 #pragma unroll
     for (int k = 0; k < 8; ++k)
-      if (32 * k + lane < left) from_f32(x + 32 * k + lane, v[k]);
+      if (32 * k + lane < left) p[32 * k + lane] = x[k];
   }
-}
-// Bytes: packed little-endian, element k of the lane in byte k % 4 of word k / 4.
-__device__ __forceinline__ void load_codes(const uint8_t* x, long long left, int lane, bool vec, uint32_t (&w)[2]) {
-  if (vec) {
-    const uint2 v = load_8(x + 8 * lane);
-    w[0] = v.x;
-    w[1] = v.y;
-  } else {
+  __device__ __forceinline__ void unpack(float2 (&out)[4]) const {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) out[k] = make_float2(x[2 * k], x[2 * k + 1]);
+  }
+  __device__ __forceinline__ void pack(const float2 (&in)[4]) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) x[2 * k] = in[k].x, x[2 * k + 1] = in[k].y;
+  }
+};
+
+template <typename T>
+struct __align__(16) Run16 {  // eight 16-bit elements, element k in half k % 2 of word k / 2
+  uint32_t w[4];
+  template <int kOffset = 0>
+  __device__ __forceinline__ void get(const T* p) {
+    const uint4 v = load_16<2 * kOffset>(p);
+    w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
+  }
+  __device__ __forceinline__ void put(T* p) const { *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]); }
+  __device__ __forceinline__ void get_some(const T* base, long long left, int lane) {
+    const uint16_t* p = reinterpret_cast<const uint16_t*>(base);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const uint32_t h = (32 * k + lane < left) ? p[32 * k + lane] : 0u;
+      w[k / 2] = k % 2 == 0 ? h : w[k / 2] | (h << 16);
+    }
+  }
+  __device__ __forceinline__ void put_some(T* base, long long left, int lane) const {
+    uint16_t* p = reinterpret_cast<uint16_t*>(base);
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+      if (32 * k + lane < left) p[32 * k + lane] = static_cast<uint16_t>(w[k / 2] >> (16 * (k % 2)));
+  }
+};
+
+template <>
+struct Run<int16_t> : Run16<int16_t> {};
+
+template <>
+struct Run<__nv_bfloat16> : Run16<__nv_bfloat16> {
+  __device__ __forceinline__ void unpack(float2 (&out)[4]) const {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) out[k] = make_float2(__uint_as_float(w[k] << 16), __uint_as_float(w[k] & 0xffff0000u));
+  }
+  __device__ __forceinline__ void pack(const float2 (&in)[4]) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const __nv_bfloat162 h = __float22bfloat162_rn(in[k]);
+      w[k] = *reinterpret_cast<const uint32_t*>(&h);
+    }
+  }
+};
+
+template <>
+struct __align__(8) Run<uint8_t> {  // element k in byte k % 4 of word k / 4
+  uint32_t w[2];
+  template <int kOffset = 0>
+  __device__ __forceinline__ void get(const uint8_t* p) {
+    const uint2 v = load_8<kOffset>(p);
+    w[0] = v.x, w[1] = v.y;
+  }
+  __device__ __forceinline__ void put(uint8_t* p) const { *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]); }
+  __device__ __forceinline__ void get_some(const uint8_t* p, long long left, int lane) {
     w[0] = w[1] = 0;
 #pragma unroll
     for (int k = 0; k < 8; ++k)
-      if (32 * k + lane < left) w[k / 4] |= static_cast<uint32_t>(x[32 * k + lane]) << (8 * (k % 4));
+      if (32 * k + lane < left) w[k / 4] |= static_cast<uint32_t>(p[32 * k + lane]) << (8 * (k % 4));
   }
-}
-__device__ __forceinline__ void store_codes(uint8_t* x, long long left, int lane, bool vec, const uint32_t (&w)[2]) {
-  if (vec) {
-    store_8(x + 8 * lane, make_uint2(w[0], w[1]));
-  } else {
+  __device__ __forceinline__ void put_some(uint8_t* p, long long left, int lane) const {
 #pragma unroll
     for (int k = 0; k < 8; ++k)
-      if (32 * k + lane < left) x[32 * k + lane] = static_cast<uint8_t>(w[k / 4] >> (8 * (k % 4)));
+      if (32 * k + lane < left) p[32 * k + lane] = static_cast<uint8_t>(w[k / 4] >> (8 * (k % 4)));
   }
+};
+
+// Two fp32 operations in one instruction, each rounded to nearest.
+#define EO_PAIR_2(name, op)                                                                                               \
+  __device__ __forceinline__ float2 name(float2 a, float2 b) {                                                             \
+    float2 d;                                                                                                              \
+    asm("{.reg .b64 a, b, d; mov.b64 a, {%2, %3}; mov.b64 b, {%4, %5}; " op ".rn.f32x2 d, a, b; mov.b64 {%0, %1}, d;}"      \
+        : "=f"(d.x), "=f"(d.y)                                                                                             \
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));                                                                         \
+    return d;                                                                                                              \
+  }
+EO_PAIR_2(mul2, "mul")
+EO_PAIR_2(add2, "add")
+#undef EO_PAIR_2
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("{.reg .b64 a, b, c, d; mov.b64 a, {%2, %3}; mov.b64 b, {%4, %5}; mov.b64 c, {%6, %7}; "
+      "fma.rn.f32x2 d, a, b, c; mov.b64 {%0, %1}, d;}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return d;
 }
-// Place, within its run, of element k of a lane.
-__device__ __forceinline__ int place_of(int k, int lane, bool vec) { return vec ? 8 * lane + k : 32 * k + lane; }
+__device__ __forceinline__ float2 both(float x) { return make_float2(x, x); }
 
 // bf16 weights whose fp32 master is kept as bf16 plus a signed 16-bit remainder: master bits = (bf16 bits << 16) +
 // remainder.  Written back as the nearest bf16 (halves away from zero, so that the remainder fits 16 bits); a NaN
 // becomes the quiet NaN with remainder zero, as adding to its payload could wrap.
-__device__ __forceinline__ void load_master(const __nv_bfloat16* p, const int16_t* r, long long left, int lane, bool vec,
-                                            float (&out)[8]) {
-  if (vec) {
-    const uint4 hi = load_16(p + 8 * lane), lo = load_16(r + 8 * lane);
-    const uint32_t h[4] = {hi.x, hi.y, hi.z, hi.w}, l[4] = {lo.x, lo.y, lo.z, lo.w};
+__device__ __forceinline__ void join_masters(const Run<__nv_bfloat16>& hi, const Run<int16_t>& lo, float2 (&out)[4]) {
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      out[2 * k] = __uint_as_float((h[k] << 16) + static_cast<uint32_t>(static_cast<int32_t>(l[k] << 16) >> 16));
-      out[2 * k + 1] = __uint_as_float((h[k] & 0xffff0000u) + static_cast<uint32_t>(static_cast<int32_t>(l[k]) >> 16));
-    }
-  } else {
-#pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      const int i = 32 * k + lane;
-      out[k] = (i < left) ? __uint_as_float((static_cast<uint32_t>(__bfloat16_as_ushort(p[i])) << 16) +
-                                            static_cast<uint32_t>(static_cast<int32_t>(r[i])))
-                          : 0.0f;
-    }
+  for (int k = 0; k < 4; ++k) {
+    out[k].x = __uint_as_float((hi.w[k] << 16) + static_cast<uint32_t>(static_cast<int32_t>(lo.w[k] << 16) >> 16));
+    out[k].y = __uint_as_float((hi.w[k] & 0xffff0000u) + static_cast<uint32_t>(static_cast<int32_t>(lo.w[k]) >> 16));
   }
 }
-__device__ __forceinline__ void split_master(float x, uint32_t& hi, uint32_t& lo) {
-  const uint32_t bits = __float_as_uint(x);
-  hi = (bits + 0x8000u) >> 16;
-  lo = bits & 0xffffu;  // bits - (hi << 16), modulo 2^16
-  if (x != x) hi = 0x7fc0u, lo = 0;
-}
-__device__ __forceinline__ void store_master(__nv_bfloat16* p, int16_t* r, long long left, int lane, bool vec,
-                                             const float (&x)[8]) {
-  uint32_t hi[8], lo[8];
+__device__ __forceinline__ void split_masters(const float2 (&x)[4], Run<__nv_bfloat16>& hi, Run<int16_t>& lo) {
 #pragma unroll
-  for (int k = 0; k < 8; ++k) split_master(x[k], hi[k], lo[k]);
-  if (vec) {
-    uint32_t h[4], l[4];
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      h[k] = hi[2 * k] | (hi[2 * k + 1] << 16);
-      l[k] = lo[2 * k] | (lo[2 * k + 1] << 16);
-    }
-    store_16(p + 8 * lane, make_uint4(h[0], h[1], h[2], h[3]));
-    store_16(r + 8 * lane, make_uint4(l[0], l[1], l[2], l[3]));
-  } else {
-#pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      const int i = 32 * k + lane;
-      if (i < left) {
-        p[i] = __ushort_as_bfloat16(static_cast<unsigned short>(hi[k]));
-        r[i] = static_cast<int16_t>(static_cast<uint16_t>(lo[k]));
-      }
-    }
+  for (int k = 0; k < 4; ++k) {
+    // a NaN as 0x7fc00000: rounding leaves it, its low half is zero
+    const uint32_t a = x[k].x != x[k].x ? 0x7fc00000u : __float_as_uint(x[k].x);
+    const uint32_t b = x[k].y != x[k].y ? 0x7fc00000u : __float_as_uint(x[k].y);
+    hi.w[k] = __byte_perm(a + 0x8000u, b + 0x8000u, 0x7632);
+    lo.w[k] = __byte_perm(a, b, 0x5410);  // bits - (hi << 16), modulo 2^16
   }
 }
 
@@ -190,6 +206,18 @@ __device__ __forceinline__ void store_master(__nv_bfloat16* p, int16_t* r, long 
 // its mean is within 1 % and its spread 7 - 13 %.
 // An unsigned value above zero never becomes code 0: it divides.  What is not finite (unsigned: or is negative) becomes
 // the code with all exponent and mantissa bits set, which no finite value reaches, and reads as NaN.
+//
+// What this costs decides the speed of the 8-bit step, and the integer pipe has half the rate of the floating-point one:
+// everything an element needs is a multiplication or an add, except the byte moves.  What is not finite is looked for
+// once per block, in the maximum that the exponent needs anyway, and dealt with off the common path.
+__device__ __forceinline__ float power_of_two(int e) {  // e in -149 .. 127
+  return __uint_as_float(e >= -126 ? static_cast<uint32_t>(e + 127) << 23 : 1u << (e + 149));
+}
+__device__ __forceinline__ float max3_nan(float a, float b, float c) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
 template <bool kSigned>
 struct Code8 {
   static constexpr int kTop = kSigned ? 14 : 30;
@@ -198,56 +226,110 @@ struct Code8 {
   static __device__ __forceinline__ float up() { return __uint_as_float(static_cast<uint32_t>(254 - kTop) << 23); }
   static __device__ __forceinline__ float down() { return __uint_as_float(static_cast<uint32_t>(kTop) << 23); }
 
-  // value of code k of a lane; scale = 2^(E - 127)
-  static __device__ __forceinline__ float decode(uint32_t word, int byte, float scale) {
-    uint32_t bits;
-    if (kSigned) {
-      bits = static_cast<uint32_t>(static_cast<int32_t>(word << (24 - 8 * byte)) >> 4) & 0x87f00000u;
-    } else {
-      bits = (byte == 3 ? word >> 4 : word << (20 - 8 * byte)) & 0x0ff00000u;
-    }
-    const float x = __fmul_rn(__fmul_rn(__uint_as_float(bits), up()), scale);
-    return ((bits & 0x0ff00000u) == (kNan << 20)) ? __uint_as_float(0x7fc00000u) : x;
-  }
-  static __device__ __forceinline__ uint32_t magnitude(float x) {  // for the block's maximum; 0 if it does not count
-    const uint32_t b = kSigned ? (__float_as_uint(x) & 0x7fffffffu) : __float_as_uint(x);
-    return b >= 0x7f800000u ? 0u : b;
-  }
-  // inv_scale = 2^(127 - E)
-  static __device__ __forceinline__ uint32_t encode(float x, float inv_scale, uint32_t d) {
-    const uint32_t b = __float_as_uint(x);
-    const float y = __fmul_rn(__fmul_rn(kSigned ? fabsf(x) : x, inv_scale), down());
-    uint32_t c = (__float_as_uint(y) + d) >> 20;
-    if (kSigned) {
-      c = ((b & 0x7fffffffu) >= 0x7f800000u) ? kNan : c;
-      return c | ((b >> 24) & 0x80u);
-    }
-    if (c == 0 && x > 0.0f) c = 1;
-    if (b == 0x80000000u) return 0;  // -0
-    return b >= 0x7f800000u ? kNan : c;
-  }
-};
-__device__ __forceinline__ float scale_of(uint32_t e) { return __uint_as_float((e == 0 ? 1u : e) << 23); }
-__device__ __forceinline__ float inv_scale_of(uint32_t e) {
-  return __uint_as_float(e >= 254u ? 0x00400000u : (254u - e) << 23);
-}
-// d = r * mul + add for a block with exponent byte e.
-struct Dither {
-  uint32_t mul, add;
-  __device__ __forceinline__ Dither(uint32_t e, bool random) {
-    mul = (random && e < 254u) ? 16u : 0u;
-    add = e >= 254u ? 0u : random ? 8u : 0x80000u;
-  }
-  __device__ __forceinline__ uint32_t operator()(uint32_t r) const { return r * mul + add; }
-};
-template <bool kSigned>
-__device__ __forceinline__ uint32_t block_exponent(const float (&x)[8]) {
-  uint32_t top = 0;
+  static __device__ __forceinline__ void decode(const Run<uint8_t>& codes, uint32_t exponent, float2 (&out)[4]) {
+    if constexpr (kSigned) {
+      // The bits are those of e4m3 (sign, 4 exponent, 3 mantissa bits, 0x7f NaN), 2^7 times as large.
+      const float2 scale = both(power_of_two(static_cast<int>(exponent) - 134));
 #pragma unroll
-  for (int k = 0; k < 8; ++k) top = max(top, Code8<kSigned>::magnitude(x[k]));
-  const uint32_t e = __reduce_max_sync(0xffffffffu, top) >> 23;
-  return e < 1u ? 1u : e;
-}
+      for (int k = 0; k < 4; ++k) {
+        uint32_t h2;
+        const uint16_t two = static_cast<uint16_t>(codes.w[k / 2] >> (16 * (k % 2)));
+        asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h2) : "h"(two));
+        out[k] = mul2(__half22float2(*reinterpret_cast<const __half2*>(&h2)), scale);
+      }
+    } else {
+      const float2 scale = both(power_of_two(static_cast<int>(exponent) - 127)), lift = both(up());
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const uint32_t w = codes.w[k / 2];
+        // the byte at bit 16, times 2^4
+        const uint32_t a = __byte_perm(w, 0, 0x4044 | (2 * (k % 2)) << 8) * 16u;
+        const uint32_t b = __byte_perm(w, 0, 0x4044 | (2 * (k % 2) + 1) << 8) * 16u;
+        out[k] = mul2(mul2(make_float2(__uint_as_float(a), __uint_as_float(b)), lift), scale);
+      }
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const uint32_t w = codes.w[j];
+        if ((~w - 0x01010101u) & w & 0x80808080u) {  // a byte is 0xff
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            if (((w >> (16 * k)) & 0xffu) == kNan) out[2 * j + k].x = __uint_as_float(0x7fc00000u);
+            if (((w >> (16 * k + 8)) & 0xffu) == kNan) out[2 * j + k].y = __uint_as_float(0x7fc00000u);
+          }
+        }
+      }
+    }
+  }
+
+  // Largest magnitude of the block as fp32 bits; at least those of infinity where something is not a number to be kept.
+  static __device__ __forceinline__ uint32_t block_top(const float (&x)[8]) {
+    uint32_t top;
+    if constexpr (kSigned) {
+      const float a = max3_nan(fabsf(x[0]), fabsf(x[1]), fabsf(x[2])), b = max3_nan(fabsf(x[3]), fabsf(x[4]), fabsf(x[5]));
+      top = __float_as_uint(max3_nan(max3_nan(a, fabsf(x[6]), fabsf(x[7])), b, b));
+    } else {
+      const uint32_t a = __vimax3_u32(__float_as_uint(x[0]), __float_as_uint(x[1]), __float_as_uint(x[2]));
+      const uint32_t b = __vimax3_u32(__float_as_uint(x[3]), __float_as_uint(x[4]), __float_as_uint(x[5]));
+      top = max(__vimax3_u32(a, __float_as_uint(x[6]), __float_as_uint(x[7])), b);
+    }
+    return __reduce_max_sync(0xffffffffu, top);
+  }
+  static __device__ __forceinline__ bool is_kept(float x) {
+    const uint32_t b = __float_as_uint(x);
+    return (kSigned ? (b & 0x7fffffffu) : b) < 0x7f800000u;
+  }
+
+  // Exponent byte and codes of a block; r[k]: sixteen random bits for each element (unused when to nearest).
+  static __device__ __forceinline__ uint32_t quantize(const float2 (&in)[4], bool random, const uint32_t (&r)[8],
+                                                      Run<uint8_t>& codes) {
+    const float x[8] = {in[0].x, in[0].y, in[1].x, in[1].y, in[2].x, in[2].y, in[3].x, in[3].y};
+    uint32_t top = block_top(x);
+    const bool special = top >= 0x7f800000u;
+    if (special) {
+      uint32_t mine = 0;
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+        if (is_kept(x[k])) mine = max(mine, __float_as_uint(x[k]) & 0x7fffffffu);
+      top = __reduce_max_sync(0xffffffffu, mine);
+    }
+    const uint32_t e = max(top >> 23, 1u);
+    const float2 inv = both(power_of_two(127 - static_cast<int>(e))), lower = both(down());
+    // 16 (bits + d) has the code in its top byte; the sign, if any, is shifted out.  The two constants make 16 d.
+    const uint32_t mul = random && e < 254u ? 256u : 0u, add = e >= 254u ? 0u : random ? 128u : 0x800000u;
+    uint32_t t[8];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const float2 y = mul2(mul2(in[k], inv), lower);
+      t[2 * k] = __float_as_uint(y.x) * 16u + (r[2 * k] * mul + add);
+      t[2 * k + 1] = __float_as_uint(y.y) * 16u + (r[2 * k + 1] * mul + add);
+      if constexpr (!kSigned) {
+        if (in[k].x > 0.0f) t[2 * k] = max(t[2 * k], 1u << 24);
+        if (in[k].y > 0.0f) t[2 * k + 1] = max(t[2 * k + 1], 1u << 24);
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      uint32_t w = __byte_perm(__byte_perm(t[4 * j], t[4 * j + 1], 0x0073), __byte_perm(t[4 * j + 2], t[4 * j + 3], 0x0073), 0x5410);
+      if constexpr (kSigned) {
+        const uint32_t signs = __byte_perm(
+            __byte_perm(__float_as_uint(x[4 * j]), __float_as_uint(x[4 * j + 1]), 0x0073),
+            __byte_perm(__float_as_uint(x[4 * j + 2]), __float_as_uint(x[4 * j + 3]), 0x0073), 0x5410);
+        w = (w & 0x7f7f7f7fu) | (signs & 0x80808080u);
+      }
+      if (special) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const uint32_t b = __float_as_uint(x[4 * j + k]);
+          if (!is_kept(x[4 * j + k]))
+            w = (w & ~(0xffu << (8 * k))) | ((!kSigned && b == 0x80000000u ? 0u : kNan | (kSigned ? (b >> 24) & 0x80u : 0u)) << (8 * k));
+        }
+      }
+      codes.w[j] = w;
+    }
+    return e;
+  }
+};
+
 // The finaliser of MurmurHash3: 32 random bits of an element from mix(key ^ element), key from (seed, tensor, step).
 __host__ __device__ __forceinline__ uint32_t mix32(uint32_t x) {
   x = (x ^ (x >> 16)) * 0x85ebca6bu;
@@ -256,6 +338,20 @@ __host__ __device__ __forceinline__ uint32_t mix32(uint32_t x) {
 }
 __host__ __device__ __forceinline__ uint32_t rounding_key(uint32_t seed, uint32_t tensor, uint32_t step) {
   return mix32(mix32(mix32(seed) ^ tensor) ^ step);
+}
+// mix32(key ^ element) of a lane's eight elements, halves apart.  The elements of a lane differ in bits below 16 only, which
+// the first step of the mixer leaves alone, so that step is done once.
+template <bool kVec>
+__device__ __forceinline__ void random_halves(uint32_t key, uint32_t first, uint32_t (&low)[8], uint32_t (&high)[8]) {
+  first ^= key;  // `first`: the lane's first element
+  first ^= first >> 16;
+#pragma unroll
+  for (int k = 0; k < 8; ++k) {
+    uint32_t x = (first ^ static_cast<uint32_t>(kVec ? k : 32 * k)) * 0x85ebca6bu;
+    x = (x ^ (x >> 13)) * 0xc2b2ae35u;
+    high[k] = x >> 16;
+    low[k] = (x ^ high[k]) & 0xffffu;
+  }
 }
 
 // ---- tables -----------------------------------------------------------------------------------------------------------
@@ -333,85 +429,257 @@ __global__ void __launch_bounds__(128)
     out[i] = adamw_factors(lr, beta1, beta2, weight_decay, method, table.t[i].step != nullptr ? *table.t[i].step : step);
 }
 
-// g, p, m, v of one lane; every operation rounded once, in this order, so that the result does not depend on how the
-// compiler would contract it (the 8-bit codes of a run must not depend on the build).
-__device__ __forceinline__ void adamw_update(float (&p)[8], const float (&g_in)[8], float (&m)[8], float (&v)[8],
+__device__ __forceinline__ float rsqrt_approx(float x) {
+  float y;
+  asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float rcp_approx(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float at_least(float x, float low) {  // NaN stays NaN
+  float y;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(x), "f"(low));
+  return y;
+}
+
+// g, p, m, v of one lane, two elements to an instruction.  Every operation is rounded once, in this order, so that the result
+// does not depend on how the compiler would contract it (the 8-bit codes of a run must not depend on the build).
+//
+// Root and quotient are rounded to nearest too, without the branches and the range checks of the compiler's, which run the
+// eight elements of a lane one after the other: one Newton step each on the hardware's approximations, its residual exact
+// through the fused multiply-add (Markstein, IBM J. Res. Dev. 34, 1990).  Compared with __fsqrt_rn on every positive float: the
+// same where the operand is at least 2^-102, within 3e-7 below; with __fdiv_rn on 3.4e10 pairs of mantissas: the same, and the
+// reciprocal inside is the nearest for every mantissa.  The root is taken of 2^24 v, so that it is exact for every normal
+// v; what overflows (v > 2^104) counts as the largest finite number, zero gives zero.  Negated operands (-v, -root,
+// -denominator) save the sign changes that the paired instructions do not have.
+__device__ __forceinline__ void adamw_update(float2 (&p)[4], const float2 (&g_in)[4], float2 (&m)[4], float2 (&v)[4],
                                              const AdamWScalars& c, const AdamWFactors& f, float grad_scale) {
+  const float2 scale = both(grad_scale), b1 = both(c.beta1), ob1 = both(c.one_minus_beta1), b2 = both(c.beta2);
+  const float2 ob2 = both(c.one_minus_beta2), l2 = both(c.l2), eps = both(-c.eps), decay = both(f.decay);
+  const float2 size = both(-f.step_size), inv = both(f.inv_root_bc2 * 0x1p-12f);
 #pragma unroll
-  for (int k = 0; k < 8; ++k) {
-    float g = __fmul_rn(g_in[k], grad_scale);
-    if (c.l2 != 0.0f) g = __fadd_rn(g, __fmul_rn(p[k], c.l2));
-    m[k] = __fadd_rn(__fmul_rn(m[k], c.beta1), __fmul_rn(g, c.one_minus_beta1));
-    v[k] = __fadd_rn(__fmul_rn(v[k], c.beta2), __fmul_rn(__fmul_rn(g, g), c.one_minus_beta2));
-    const float denom = __fadd_rn(__fmul_rn(__fsqrt_rn(v[k]), f.inv_root_bc2), c.eps);
-    p[k] = __fsub_rn(__fmul_rn(p[k], f.decay), __fmul_rn(__fdiv_rn(m[k], denom), f.step_size));
+  for (int k = 0; k < 4; ++k) {
+    float2 g = mul2(g_in[k], scale);
+    if (c.l2 != 0.0f) g = add2(g, mul2(p[k], l2));
+    m[k] = add2(mul2(m[k], b1), mul2(g, ob1));
+    v[k] = add2(mul2(v[k], b2), mul2(mul2(g, g), ob2));
+    float2 nv = mul2(v[k], both(-0x1p24f));
+    nv.x = at_least(nv.x, -3.4028234664e38f);
+    nv.y = at_least(nv.y, -3.4028234664e38f);
+    const float2 above_zero = add2(nv, both(-0x1p-126f));
+    const float2 y = make_float2(rsqrt_approx(-above_zero.x), rsqrt_approx(-above_zero.y));
+    float2 nroot = mul2(nv, y);
+    nroot = fma2(fma2(nroot, nroot, nv), mul2(y, both(0.5f)), nroot);
+    const float2 nd = add2(mul2(nroot, inv), eps);
+    float2 z = make_float2(rcp_approx(-nd.x), rcp_approx(-nd.y));
+    z = fma2(z, fma2(nd, z, both(1.0f)), z);
+    float2 q = mul2(m[k], z);
+    q = fma2(fma2(nd, q, m[k]), z, q);
+    p[k] = add2(mul2(p[k], decay), mul2(q, size));
   }
 }
 
+// The eight elements of a lane: parameters, gradients, moments as they lie in memory.
+template <typename P, typename G, bool kRemainder, bool k8>
+struct AdamWRun {
+  using Moment = typename std::conditional<k8, uint8_t, float>::type;
+  Run<P> p;
+  Run<G> g;
+  Run<Moment> m, v;
+  Run<int16_t> r;
+  uint32_t me, ve;
+
+  // kVec, first: as the lane's elements lie, and the index of its first one (random rounding).
+  template <bool kVec>
+  __device__ __forceinline__ void step(const AdamWScalars& c, const AdamWFactors& f, float grad_scale, uint32_t key,
+                                       uint32_t first) {
+    float2 xp[4], xg[4], xm[4], xv[4];
+    g.unpack(xg);
+    if constexpr (kRemainder) join_masters(p, r, xp); else p.unpack(xp);
+    if constexpr (k8) {
+      Code8<true>::decode(m, me, xm);
+      Code8<false>::decode(v, ve, xv);
+    } else {
+      m.unpack(xm);
+      v.unpack(xv);
+    }
+    adamw_update(xp, xg, xm, xv, c, f, grad_scale);
+    if constexpr (kRemainder) split_masters(xp, p, r); else p.pack(xp);
+    if constexpr (k8) {
+      uint32_t low[8], high[8];
+      random_halves<kVec>(key, first, low, high);
+      me = Code8<true>::quantize(xm, true, low, m);
+      ve = Code8<false>::quantize(xv, true, high, v);
+    } else {
+      m.pack(xm);
+      v.pack(xv);
+    }
+  }
+};
+
+// Addresses of a lane's elements in whole, aligned runs; they move on by one trip.
+template <typename P, typename G, bool kRemainder, bool k8>
+struct AdamWCursor {
+  using Data = AdamWRun<P, G, kRemainder, k8>;
+  using Moment = typename Data::Moment;
+  P* p;
+  const G* g;
+  Moment *m, *v;
+  int16_t* r;
+  __device__ __forceinline__ AdamWCursor(const AdamWEntry& t, long long at, int lane)
+      : p(static_cast<P*>(t.p) + at + 8 * lane),
+        g(static_cast<const G*>(t.g) + at + 8 * lane),
+        m(static_cast<Moment*>(t.m) + at + 8 * lane),
+        v(static_cast<Moment*>(t.v) + at + 8 * lane),
+        r(t.r + at + 8 * lane) {}
+  __device__ __forceinline__ void get(Data& d) const {
+    d.g.get(g);
+    d.p.get(p);
+    d.m.get(m);
+    d.v.get(v);
+    if constexpr (kRemainder) d.r.get(r);
+  }
+  __device__ __forceinline__ void put(const Data& d) const {
+    d.p.put(p);
+    if constexpr (kRemainder) d.r.put(r);
+    d.m.put(m);
+    d.v.put(v);
+  }
+  __device__ __forceinline__ void next() {
+    p += kOptTrip, g += kOptTrip, m += kOptTrip, v += kOptTrip;
+    if constexpr (kRemainder) r += kOptTrip;
+  }
+};
+
+// Runs of the 8-bit step on their way through shared memory: a warp's own ring of kRingStages runs, filled by asynchronous copies
+// several trips ahead.  The step keeps about 60 instructions an element between a load and its store, at 24 warps an SM too few
+// bytes are in flight otherwise.
+constexpr int kRingStages = 4;
+template <typename P, typename G, bool kRemainder>
+struct AdamWRing {
+  static constexpr int kP = 0, kG = kP + kOptRun * sizeof(P), kM = kG + kOptRun * sizeof(G), kV = kM + kOptRun,
+                       kR = kV + kOptRun, kBytes = kR + (kRemainder ? 2 * kOptRun : 0);
+  static constexpr int kCtaBytes = kBytes * kRingStages * (kOptThreads / 32);
+
+  template <int kRunBytes>
+  static __device__ __forceinline__ void copy(uint32_t to, const void* run, int lane) {
+    constexpr int kPiece = kRunBytes >= 512 ? 16 : 8;
+    const char* from = static_cast<const char*>(run) + kPiece * lane;
+#pragma unroll
+    for (int at = 0; at < kRunBytes; at += 32 * kPiece) {
+      if constexpr (kPiece == 16)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to + at + kPiece * lane), "l"(from + at) : "memory");
+      else
+        asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(to + at + kPiece * lane), "l"(from + at) : "memory");
+    }
+  }
+  // `at`: first element of the run
+  static __device__ __forceinline__ void fetch(uint32_t stage, const AdamWEntry& t, long long at, int lane) {
+    copy<kOptRun * sizeof(P)>(stage + kP, static_cast<const P*>(t.p) + at, lane);
+    copy<kOptRun * sizeof(G)>(stage + kG, static_cast<const G*>(t.g) + at, lane);
+    copy<kOptRun>(stage + kM, static_cast<const uint8_t*>(t.m) + at, lane);
+    copy<kOptRun>(stage + kV, static_cast<const uint8_t*>(t.v) + at, lane);
+    if constexpr (kRemainder) copy<kOptRun * 2>(stage + kR, t.r + at, lane);
+  }
+  static __device__ __forceinline__ void read(const char* stage, int lane, AdamWRun<P, G, kRemainder, true>& d) {
+    d.p = reinterpret_cast<const Run<P>*>(stage + kP)[lane];
+    d.g = reinterpret_cast<const Run<G>*>(stage + kG)[lane];
+    d.m = reinterpret_cast<const Run<uint8_t>*>(stage + kM)[lane];
+    d.v = reinterpret_cast<const Run<uint8_t>*>(stage + kV)[lane];
+    if constexpr (kRemainder) d.r = reinterpret_cast<const Run<int16_t>*>(stage + kR)[lane];
+  }
+};
+
 // kRemainder: p is bf16 with remainders.  k8: m and v are codes with exponent bytes.
+// Bound by HBM with fp32 moments (28 bytes an element: 99 % of the copy bandwidth on 268 M elements, bf16 types 95 %).  With
+// 8-bit moments an element costs about 55 instructions for its 10 to 16 bytes: 97 % (fp32 types), 94 % (bf16 gradients), 89 %
+// (bf16 with remainders) and 71 % (bf16), the last bound by the issue slots.  Three CTAs an SM (80 registers): two are 6 - 12 %
+// slower with bf16 types, four spill.
 template <typename P, typename G, bool kRemainder, bool k8, int kCapacity>
-__global__ void __launch_bounds__(kOptThreads)
+__global__ void __launch_bounds__(kOptThreads, 3)
     adamw_kernel(const __grid_constant__ TensorTable<AdamWEntry, kCapacity> table, const __grid_constant__ AdamWScalars c) {
+  using Data = AdamWRun<P, G, kRemainder, k8>;
+  using Moment = typename Data::Moment;
   const int which = find_tensor(table, blockIdx.x);
   const AdamWEntry& t = table.t[which];
   const AdamWFactors f = c.dev_factors != nullptr ? c.dev_factors[which] : c.f;
   const float grad_scale = c.grad_scale != nullptr ? *c.grad_scale : 1.0f;
   const uint32_t key = k8 ? rounding_key(c.seed, t.index, f.step) : 0u;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const long long numel = t.numel;
-  long long at = (static_cast<long long>(blockIdx.x - table.first[which]) * table.trips) * kOptTrip + warp * kOptRun;
-  P* const tp = static_cast<P*>(t.p);
-  const G* const tg = static_cast<const G*>(t.g);
-  for (int trip = 0; trip < table.trips && at < numel; ++trip, at += kOptTrip) {
-    const long long left = numel - at;
-    const bool vec = t.vec != 0 && left >= kOptRun;
-    float p[8], g[8], m[8], v[8];
-    load_lane(tg + at, left, lane, vec, g);
-    if constexpr (kRemainder) {
-      load_master(tp + at, t.r + at, left, lane, vec, p);
-    } else {
-      load_lane(tp + at, left, lane, vec, p);
-    }
+  const long long begin = static_cast<long long>(blockIdx.x - table.first[which]) * table.trips * kOptTrip;
+  const long long end = min(begin + static_cast<long long>(table.trips) * kOptTrip, t.numel);
+  long long at = begin + warp * kOptRun;
+  if (t.vec) {
+    const int whole = end - at >= kOptRun ? static_cast<int>((end - at - kOptRun) / kOptTrip) + 1 : 0;
+    AdamWCursor<P, G, kRemainder, k8> cursor(t, at, lane);
+    Data data;
     if constexpr (k8) {
-      uint32_t cm[2], cv[2];
-      load_codes(static_cast<uint8_t*>(t.m) + at, left, lane, vec, cm);
-      load_codes(static_cast<uint8_t*>(t.v) + at, left, lane, vec, cv);
-      const float sm = scale_of(t.me[at / kOptRun]), sv = scale_of(t.ve[at / kOptRun]);
-#pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        m[k] = Code8<true>::decode(cm[k / 4], k % 4, sm);
-        v[k] = Code8<false>::decode(cv[k / 4], k % 4, sv);
+      using Ring = AdamWRing<P, G, kRemainder>;
+      extern __shared__ __align__(16) char ring_bytes[];
+      const char* ring = ring_bytes + warp * (Ring::kBytes * kRingStages);
+      const uint32_t ring_at = static_cast<uint32_t>(__cvta_generic_to_shared(ring));
+      uint8_t *me = t.me + at / kOptRun, *ve = t.ve + at / kOptRun;
+      uint32_t mes = 0, ves = 0;  // lane l: the exponents of the warp's run l from here
+      for (int i = 0; i < kRingStages - 1; ++i) {
+        if (i < whole) Ring::fetch(ring_at + i * Ring::kBytes, t, at + static_cast<long long>(i) * kOptTrip, lane);
+        asm volatile("cp.async.commit_group;" ::: "memory");
+      }
+      int stage = 0;
+      for (int i = 0; i < whole; ++i, at += kOptTrip, cursor.next()) {
+        if ((i & 31) == 0 && i + lane < whole) {
+          mes = me[(i + lane) * (kOptTrip / kOptRun)];
+          ves = ve[(i + lane) * (kOptTrip / kOptRun)];
+        }
+        asm volatile("cp.async.wait_group %0;" ::"n"(kRingStages - 2) : "memory");
+        __syncwarp();  // the run is there for all lanes, and all of them have read the one whose place is filled next
+        Ring::read(ring + stage * Ring::kBytes, lane, data);
+        if (i + kRingStages - 1 < whole)
+          Ring::fetch(ring_at + (stage == 0 ? kRingStages - 1 : stage - 1) * Ring::kBytes, t, at + (kRingStages - 1) * static_cast<long long>(kOptTrip), lane);
+        asm volatile("cp.async.commit_group;" ::: "memory");
+        stage = stage == kRingStages - 1 ? 0 : stage + 1;
+        data.me = __shfl_sync(0xffffffffu, mes, i & 31);
+        data.ve = __shfl_sync(0xffffffffu, ves, i & 31);
+        data.template step<true>(c, f, grad_scale, key, static_cast<uint32_t>(at) + 8 * lane);
+        cursor.put(data);
+        if (lane == 0) {
+          me[i * (kOptTrip / kOptRun)] = static_cast<uint8_t>(data.me);
+          ve[i * (kOptTrip / kOptRun)] = static_cast<uint8_t>(data.ve);
+        }
       }
     } else {
-      load_lane(static_cast<const float*>(t.m) + at, left, lane, vec, m);
-      load_lane(static_cast<const float*>(t.v) + at, left, lane, vec, v);
-    }
-    adamw_update(p, g, m, v, c, f, grad_scale);
-    if constexpr (kRemainder) {
-      store_master(tp + at, t.r + at, left, lane, vec, p);
-    } else {
-      store_lane(tp + at, left, lane, vec, p);
-    }
-    if constexpr (k8) {
-      const uint32_t em = block_exponent<true>(m), ev = block_exponent<false>(v);
-      const float im = inv_scale_of(em), iv = inv_scale_of(ev);
-      const Dither dm(em, true), dv(ev, true);
-      uint32_t cm[2] = {0, 0}, cv[2] = {0, 0};
-#pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        const uint32_t r = mix32(key ^ static_cast<uint32_t>(at + place_of(k, lane, vec)));
-        cm[k / 4] |= Code8<true>::encode(m[k], im, dm(r & 0xffffu)) << (8 * (k % 4));
-        cv[k / 4] |= Code8<false>::encode(v[k], iv, dv(r >> 16)) << (8 * (k % 4));
+      for (int i = 0; i < whole; ++i, at += kOptTrip, cursor.next()) {
+        cursor.get(data);
+        data.template step<true>(c, f, grad_scale, key, 0u);
+        cursor.put(data);
       }
-      store_codes(static_cast<uint8_t*>(t.m) + at, left, lane, vec, cm);
-      store_codes(static_cast<uint8_t*>(t.v) + at, left, lane, vec, cv);
+    }
+  }
+  for (; at < end; at += kOptTrip) {
+    const long long left = end - at;
+    Data data;
+    data.g.get_some(static_cast<const G*>(t.g) + at, left, lane);
+    data.p.get_some(static_cast<const P*>(t.p) + at, left, lane);
+    data.m.get_some(static_cast<const Moment*>(t.m) + at, left, lane);
+    data.v.get_some(static_cast<const Moment*>(t.v) + at, left, lane);
+    if constexpr (kRemainder) data.r.get_some(t.r + at, left, lane);
+    if constexpr (k8) {
+      data.me = t.me[at / kOptRun];
+      data.ve = t.ve[at / kOptRun];
+    }
+    data.template step<false>(c, f, grad_scale, key, static_cast<uint32_t>(at) + lane);
+    data.p.put_some(static_cast<P*>(t.p) + at, left, lane);
+    if constexpr (kRemainder) data.r.put_some(t.r + at, left, lane);
+    data.m.put_some(static_cast<Moment*>(t.m) + at, left, lane);
+    data.v.put_some(static_cast<Moment*>(t.v) + at, left, lane);
+    if constexpr (k8) {
+      __syncwarp();  // every lane has read the exponents
       if (lane == 0) {
-        t.me[at / kOptRun] = static_cast<uint8_t>(em);
-        t.ve[at / kOptRun] = static_cast<uint8_t>(ev);
+        t.me[at / kOptRun] = static_cast<uint8_t>(data.me);
+        t.ve[at / kOptRun] = static_cast<uint8_t>(data.ve);
       }
-    } else {
-      store_lane(static_cast<float*>(t.m) + at, left, lane, vec, m);
-      store_lane(static_cast<float*>(t.v) + at, left, lane, vec, v);
     }
   }
 }
@@ -424,23 +692,63 @@ struct GradEntry {
   uint32_t vec;
 };
 
-// partial[chunk] = sum of squares of the chunk, in float64 (the squares of fp32 gradients leave the fp32 range) and in a
-// fixed order.
+// Sum of squares of a lane's eight elements in float64.  Squares of fp32 gradients leave the fp32 range, so fp32 may
+// be used only where they stay well inside it: there pairs of them are added in fp32 (one rounding each) and half the
+// conversions to float64 are saved, which run at an eighth of the rate of the additions and bound the sum of bf16 gradients.
+__device__ __forceinline__ double sum_of_squares(const float2 (&g)[4]) {
+  float2 s[4];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) s[k] = mul2(g[k], g[k]);
+  const float2 a = add2(s[0], s[1]), b = add2(s[2], s[3]);
+  const float top = fmaxf(fmaxf(a.x, a.y), fmaxf(b.x, b.y));
+  if (top > 0x1p-80f && top < 0x1p120f)
+    return (static_cast<double>(a.x) + static_cast<double>(a.y)) + (static_cast<double>(b.x) + static_cast<double>(b.y));
+  double sum = 0.0;
+#pragma unroll
+  for (int k = 0; k < 4; ++k)
+    sum += static_cast<double>(g[k].x) * g[k].x + static_cast<double>(g[k].y) * g[k].y;
+  return sum;
+}
+
+// partial[chunk] = sum of squares of the chunk, in a fixed order.
 template <typename G, int kCapacity>
 __global__ void __launch_bounds__(kOptThreads)
     grad_sumsq_kernel(const __grid_constant__ TensorTable<GradEntry, kCapacity> table, double* __restrict__ partial) {
   const int which = find_tensor(table, blockIdx.x);
   const GradEntry& t = table.t[which];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const long long numel = t.numel;
-  long long at = (static_cast<long long>(blockIdx.x - table.first[which]) * table.trips) * kOptTrip + warp * kOptRun;
+  const long long begin = static_cast<long long>(blockIdx.x - table.first[which]) * table.trips * kOptTrip;
+  const long long end = min(begin + static_cast<long long>(table.trips) * kOptTrip, t.numel);
+  long long at = begin + warp * kOptRun;
   const G* const tg = static_cast<const G*>(t.g);
   double acc = 0.0;
-  for (int trip = 0; trip < table.trips && at < numel; ++trip, at += kOptTrip) {
-    float g[8];
-    load_lane(tg + at, numel - at, lane, t.vec != 0 && numel - at >= kOptRun, g);
+  float2 g[4];
+  if (t.vec) {
+    const G* p = tg + at + 8 * lane;
+    for (; at + 3 * kOptTrip + kOptRun <= end; at += 4 * kOptTrip, p += 4 * kOptTrip) {  // four loads in flight
+      Run<G> run[4];
+      run[0].get(p);
+      run[1].template get<kOptTrip>(p);
+      run[2].template get<2 * kOptTrip>(p);
+      run[3].template get<3 * kOptTrip>(p);
 #pragma unroll
-    for (int k = 0; k < 8; ++k) acc += static_cast<double>(g[k]) * g[k];
+      for (int i = 0; i < 4; ++i) {
+        run[i].unpack(g);
+        acc += sum_of_squares(g);
+      }
+    }
+    for (; at + kOptRun <= end; at += kOptTrip, p += kOptTrip) {
+      Run<G> run;
+      run.get(p);
+      run.unpack(g);
+      acc += sum_of_squares(g);
+    }
+  }
+  for (; at < end; at += kOptTrip) {
+    Run<G> run;
+    run.get_some(tg + at, end - at, lane);
+    run.unpack(g);
+    acc += sum_of_squares(g);
   }
   const double total = block_reduce_sum(acc);
   if (threadIdx.x == 0) partial[blockIdx.x] = total;
@@ -469,45 +777,86 @@ __global__ void __launch_bounds__(kOptThreads)
   const int which = find_tensor(table, blockIdx.x);
   const GradEntry& t = table.t[which];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const long long numel = t.numel;
-  long long at = (static_cast<long long>(blockIdx.x - table.first[which]) * table.trips) * kOptTrip + warp * kOptRun;
+  const long long begin = static_cast<long long>(blockIdx.x - table.first[which]) * table.trips * kOptTrip;
+  const long long end = min(begin + static_cast<long long>(table.trips) * kOptTrip, t.numel);
+  long long at = begin + warp * kOptRun;
   G* const tg = static_cast<G*>(t.g);
-  for (int trip = 0; trip < table.trips && at < numel; ++trip, at += kOptTrip) {
-    const long long left = numel - at;
-    const bool vec = t.vec != 0 && left >= kOptRun;
-    float g[8];
-    load_lane(static_cast<const G*>(tg) + at, left, lane, vec, g);
+  auto scale = [coef](Run<G>& run) {
+    float2 g[4];
+    run.unpack(g);
 #pragma unroll
-    for (int k = 0; k < 8; ++k) g[k] = __fmul_rn(g[k], coef);
-    store_lane(tg + at, left, lane, vec, g);
+    for (int k = 0; k < 4; ++k) g[k] = mul2(g[k], both(coef));
+    run.pack(g);
+  };
+  if (t.vec) {
+    G* p = tg + at + 8 * lane;
+    for (; at + kOptTrip + kOptRun <= end; at += 2 * kOptTrip, p += 2 * kOptTrip) {  // two loads in flight
+      Run<G> a, b;
+      a.get(p);
+      b.template get<kOptTrip>(p);
+      scale(a);
+      a.put(p);
+      scale(b);
+      b.put(p + kOptTrip);
+    }
+    for (; at + kOptRun <= end; at += kOptTrip, p += kOptTrip) {
+      Run<G> run;
+      run.get(p);
+      scale(run);
+      run.put(p);
+    }
+  }
+  for (; at < end; at += kOptTrip) {
+    Run<G> run;
+    run.get_some(tg + at, end - at, lane);
+    scale(run);
+    run.put_some(tg + at, end - at, lane);
   }
 }
 
 // ---- block quantiser --------------------------------------------------------------------------------------------------
+// A warp takes kQuantRuns blocks, all of them read before the first is worked on.
 
-// One warp per block of 256.  `random`: stochastic rounding with `key`, else to nearest (halves away from zero).
+constexpr int kQuantRuns = 4;
+constexpr int kQuantChunk = kQuantRuns * kOptTrip;  // elements of a CTA
+
+// `random`: stochastic rounding with `key`, else to nearest (halves away from zero).
 template <typename T, bool kSigned>
 __global__ void __launch_bounds__(kOptThreads)
     quantize_kernel(const T* __restrict__ x, long long numel, int aligned, int random, uint32_t key,
                     uint8_t* __restrict__ codes, uint8_t* __restrict__ exponents) {
   const int lane = threadIdx.x & 31;
-  const long long block = static_cast<long long>(blockIdx.x) * (kOptThreads / 32) + (threadIdx.x >> 5);
-  const long long at = block * kOptRun, left = numel - at;
-  if (left <= 0) return;
-  const bool vec = aligned && left >= kOptRun;
-  float v[8];
-  load_lane(x + at, left, lane, vec, v);
-  const uint32_t e = block_exponent<kSigned>(v);
-  const float inv = inv_scale_of(e);
-  const Dither d(e, random != 0);
-  uint32_t w[2] = {0, 0};
+  const long long begin = static_cast<long long>(blockIdx.x) * kQuantChunk + (threadIdx.x >> 5) * kOptRun;
+  uint32_t low[8], high[8];
+  float2 v[4];
+  Run<uint8_t> out;
+  if (aligned && begin + (kQuantRuns - 1) * kOptTrip + kOptRun <= numel) {
+    Run<T> run[kQuantRuns];
+    const T* p = x + begin + 8 * lane;
+    run[0].get(p);
+    run[1].template get<kOptTrip>(p);
+    run[2].template get<2 * kOptTrip>(p);
+    run[3].template get<3 * kOptTrip>(p);
 #pragma unroll
-  for (int k = 0; k < 8; ++k) {
-    const uint32_t r = mix32(key ^ static_cast<uint32_t>(at + place_of(k, lane, vec)));
-    w[k / 4] |= Code8<kSigned>::encode(v[k], inv, d(kSigned ? (r & 0xffffu) : (r >> 16))) << (8 * (k % 4));
+    for (int i = 0; i < kQuantRuns; ++i) {
+      const long long at = begin + i * kOptTrip;
+      run[i].unpack(v);
+      random_halves<true>(key, static_cast<uint32_t>(at) + 8 * lane, low, high);
+      const uint32_t e = Code8<kSigned>::quantize(v, random != 0, kSigned ? low : high, out);
+      out.put(codes + at + 8 * lane);
+      if (lane == 0) exponents[at / kOptRun] = static_cast<uint8_t>(e);
+    }
+    return;
   }
-  store_codes(codes + at, left, lane, vec, w);
-  if (lane == 0) exponents[block] = static_cast<uint8_t>(e);
+  for (long long at = begin; at < numel && at < begin + kQuantChunk; at += kOptTrip) {
+    Run<T> run;
+    run.get_some(x + at, numel - at, lane);
+    run.unpack(v);
+    random_halves<false>(key, static_cast<uint32_t>(at) + lane, low, high);
+    const uint32_t e = Code8<kSigned>::quantize(v, random != 0, kSigned ? low : high, out);
+    out.put_some(codes + at, numel - at, lane);
+    if (lane == 0) exponents[at / kOptRun] = static_cast<uint8_t>(e);
+  }
 }
 
 template <typename T, bool kSigned>
@@ -515,17 +864,34 @@ __global__ void __launch_bounds__(kOptThreads)
     dequantize_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ exponents, long long numel, int aligned,
                       T* __restrict__ out) {
   const int lane = threadIdx.x & 31;
-  const long long block = static_cast<long long>(blockIdx.x) * (kOptThreads / 32) + (threadIdx.x >> 5);
-  const long long at = block * kOptRun, left = numel - at;
-  if (left <= 0) return;
-  const bool vec = aligned && left >= kOptRun;
-  uint32_t w[2];
-  load_codes(codes + at, left, lane, vec, w);
-  const float scale = scale_of(exponents[block]);
-  float v[8];
+  const long long begin = static_cast<long long>(blockIdx.x) * kQuantChunk + (threadIdx.x >> 5) * kOptRun;
+  float2 v[4];
+  Run<T> run;
+  if (aligned && begin + (kQuantRuns - 1) * kOptTrip + kOptRun <= numel) {
+    Run<uint8_t> in[kQuantRuns];
+    uint32_t e[kQuantRuns];
+    const uint8_t* p = codes + begin + 8 * lane;
+    in[0].get(p);
+    in[1].template get<kOptTrip>(p);
+    in[2].template get<2 * kOptTrip>(p);
+    in[3].template get<3 * kOptTrip>(p);
 #pragma unroll
-  for (int k = 0; k < 8; ++k) v[k] = Code8<kSigned>::decode(w[k / 4], k % 4, scale);
-  store_lane(out + at, left, lane, vec, v);
+    for (int i = 0; i < kQuantRuns; ++i) e[i] = exponents[(begin + i * kOptTrip) / kOptRun];
+#pragma unroll
+    for (int i = 0; i < kQuantRuns; ++i) {
+      Code8<kSigned>::decode(in[i], e[i], v);
+      run.pack(v);
+      run.put(out + begin + i * kOptTrip + 8 * lane);
+    }
+    return;
+  }
+  for (long long at = begin; at < numel && at < begin + kQuantChunk; at += kOptTrip) {
+    Run<uint8_t> in;
+    in.get_some(codes + at, numel - at, lane);
+    Code8<kSigned>::decode(in, exponents[at / kOptRun], v);
+    run.pack(v);
+    run.put_some(out + at, numel - at, lane);
+  }
 }
 
 }  // namespace eo
