@@ -9,7 +9,6 @@ from __future__ import annotations
 import ctypes
 import os
 import struct
-from array import array
 from ctypes import POINTER, c_char_p, c_double, c_float, c_int, c_int64, c_size_t, c_uint32, c_void_p
 
 import torch
@@ -114,9 +113,9 @@ _PROTOTYPES: dict[str, tuple] = {
         + [c_int, c_int, c_int, c_float, c_float, c_void_p],
     ),
     "eo_adamw_scratch_bytes": (c_size_t, [c_int]),
-    "eo_adamw_step": (c_int, [c_int, c_void_p, c_char_p, c_void_p]),
+    "eo_adamw_step": (c_int, [c_int, c_char_p, c_char_p, c_void_p]),
     "eo_grad_norm_scratch_bytes": (c_size_t, [c_int]),
-    "eo_grad_norm": (c_int, [c_int, c_void_p, c_float, c_int, c_void_p, c_void_p, c_size_t, c_void_p]),
+    "eo_grad_norm": (c_int, [c_int, c_char_p, c_float, c_int, c_void_p, c_void_p, c_size_t, c_void_p]),
     "eo_quantize_blockwise": (
         c_int,
         [c_void_p, c_int, c_int64, c_int, c_int, c_uint32, c_void_p, c_void_p, c_void_p],
@@ -772,31 +771,48 @@ def peek_device_status_async(pinned: torch.Tensor, device: torch.device) -> None
 MAX_TENSORS_PER_LAUNCH = 384
 QUANT_BLOCK = 256
 
-KIND_PARAM_BF16, KIND_GRAD_BF16, KIND_REMAINDER = 1, 2, 4
 _DECAY_METHODS = {"decoupled": 0, "independent": 1, "palm": 2, "l2": 3}
 _CONFIG = struct.Struct("<dddddqQQQQiiII")  # eo_adamw_config
+_host_module = None
+
+
+def host():
+    """The module that checks lists of tensors and builds the tables of their addresses (``csrc/host_tables.cpp``)."""
+    global _host_module
+    if _host_module is None:
+        try:
+            from emerging_optimizers_b200 import _host
+        except ImportError as e:
+            raise NativeLibraryError(
+                f"the host module cannot be loaded ({e}): build it with `python -m emerging_optimizers_b200.build`"
+            ) from e
+        if _host.TORCH_VERSION != torch.__version__.split("+")[0]:
+            raise NativeLibraryError(
+                f"the host module was built for torch {_host.TORCH_VERSION}, this is {torch.__version__}: build it again "
+                "with `python -m emerging_optimizers_b200.build --force`"
+            )
+        _host_module = _host
+    return _host_module
 
 
 def _launch(device: int, call, *args) -> int:
     """``call(*args, stream)`` with ``device`` current, on its current stream."""
-    if torch.cuda.current_device() == device:
-        return call(*args, torch.cuda.current_stream(device).cuda_stream)
+    stream, is_current, _ = host().stream(device)
+    if is_current:
+        return call(*args, stream)
     with torch.cuda.device(device):
-        return call(*args, torch.cuda.current_stream(device).cuda_stream)
+        return call(*args, stream)
 
 
 def adamw_step(
-    device: int, columns: list[list[int]], *, lr: float, betas: tuple[float, float], eps: float, weight_decay: float,
-    method: str, step: int, state_bits: int, seed: int = 0, first_index: int = 0, lr_tensor: torch.Tensor | None = None,
-    grad_scale: torch.Tensor | None = None,
+    device: int, n: int, table: bytes, kinds: int, *, lr: float, betas: tuple[float, float], eps: float,
+    weight_decay: float, method: str, step: int, on_device: bool, state_bits: int, seed: int = 0, first_index: int = 0,
+    lr_tensor: torch.Tensor | None = None, grad_scale: torch.Tensor | None = None,
 ) -> None:  # fmt: skip
-    """One AdamW step; ``columns`` are the ten rows of ``eo_adamw_step``'s table, one integer per tensor."""
+    """One AdamW step of the ``n`` tensors of ``table`` (see ``eo_adamw_step``); ``kinds`` is the set of kinds in it, as bits;
+    ``on_device``: the step counters or the learning rate are read from device memory."""
     global launch_count
-    n = len(columns[0])
-    table = array("q")
-    for column in columns:
-        table.extend(column)
-    scratch, scratch_ptr, nbytes, on_device = None, 0, 0, lr_tensor is not None or any(columns[7])
+    scratch, scratch_ptr, nbytes = None, 0, 0
     if on_device:
         nbytes = lib().eo_adamw_scratch_bytes(n)
         scratch = torch.empty(nbytes, dtype=torch.uint8, device=f"cuda:{device}")
@@ -806,27 +822,23 @@ def adamw_step(
         lr_tensor.data_ptr() if lr_tensor is not None else 0, grad_scale.data_ptr() if grad_scale is not None else 0,
         scratch_ptr, nbytes, _DECAY_METHODS[method], state_bits, seed, first_index,
     )  # fmt: skip
-    launch_count += len(set(columns[9])) * -(-n // MAX_TENSORS_PER_LAUNCH) * (2 if on_device else 1)
-    rc = _launch(device, lib().eo_adamw_step, n, table.buffer_info()[0], config)
-    _check(rc, "eo_adamw_step")
+    launch_count += kinds.bit_count() * -(-n // MAX_TENSORS_PER_LAUNCH) * (2 if on_device else 1)
+    _check(_launch(device, lib().eo_adamw_step, n, table, config), "eo_adamw_step")
 
 
-def grad_norm(device: int, columns: list[list[int]], max_norm: float, in_place: bool) -> torch.Tensor:
-    """Norm and clipping coefficient (fp32, shape (2,)) of the tensors of ``columns`` (addresses, element counts,
-    1 for bf16); ``in_place`` also multiplies them by the coefficient.  See ``eo_grad_norm``."""
+def grad_norm(
+    index: int, device: torch.device, n: int, table: bytes, types: int, max_norm: float, in_place: bool
+) -> torch.Tensor:
+    """Norm and clipping coefficient (fp32, shape (2,)) of the ``n`` tensors of ``table`` (see ``eo_grad_norm``);
+    ``types`` is the set of types in it, as bits; ``in_place`` also multiplies them by the coefficient."""
     global launch_count
-    n = len(columns[0])
-    table = array("q")
-    for column in columns:
-        table.extend(column)
-    out = torch.empty(2, dtype=torch.float32, device=f"cuda:{device}")
+    out = torch.empty(2, dtype=torch.float32, device=device)
     nbytes = lib().eo_grad_norm_scratch_bytes(n)
-    scratch = torch.empty(nbytes, dtype=torch.uint8, device=out.device)
-    launch_count += 1 + len(set(columns[2])) * -(-n // MAX_TENSORS_PER_LAUNCH) * (2 if in_place else 1)
+    scratch = torch.empty(nbytes, dtype=torch.uint8, device=device)
+    launch_count += 1 + types.bit_count() * -(-n // MAX_TENSORS_PER_LAUNCH) * (2 if in_place else 1)
     rc = _launch(
-        device, lib().eo_grad_norm, n, table.buffer_info()[0], max_norm, 1 if in_place else 0, out.data_ptr(),
-        scratch.data_ptr(), nbytes,
-    )  # fmt: skip
+        index, lib().eo_grad_norm, n, table, max_norm, 1 if in_place else 0, out.data_ptr(), scratch.data_ptr(), nbytes
+    )
     _check(rc, "eo_grad_norm")
     return out
 

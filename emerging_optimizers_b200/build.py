@@ -1,4 +1,5 @@
-"""Build ``libeo_b200.so`` in-tree with nvcc for sm_100a (cross-compiles without a GPU).
+"""Build ``libeo_b200.so`` in-tree with nvcc for sm_100a (cross-compiles without a GPU), and the Python extension
+``_host.so`` (tables of tensor addresses, ``csrc/host_tables.cpp``) with g++ against the installed torch.
 
 Usage: ``python -m emerging_optimizers_b200.build [--force] [--verbose]``
 """
@@ -10,12 +11,15 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 
 
 PKG_DIR = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(PKG_DIR, "csrc")
 OUT = os.path.join(PKG_DIR, "libeo_b200.so")
 SOURCES = ["eo_b200.cu"]
+HOST_OUT = os.path.join(PKG_DIR, "_host.so")
+HOST_SOURCE = os.path.join(CSRC, "host_tables.cpp")
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
     "-O3", "-std=c++17", "-lineinfo",
@@ -46,23 +50,51 @@ def needs_build() -> bool:
     return any(os.path.getmtime(f) > built for f in _inputs())
 
 
+def _run(cmd: list[str], tmp: str, out: str) -> str:
+    """Run a compiler that writes ``tmp`` and move the result to ``out``: a reader never sees a half-written file."""
+    res = subprocess.run(cmd, capture_output=True, text=True)
+    if res.returncode != 0:
+        if os.path.exists(tmp):
+            os.remove(tmp)
+        raise RuntimeError(f"{os.path.basename(cmd[0])} failed:\n{' '.join(cmd)}\n{res.stdout}\n{res.stderr}")
+    os.replace(tmp, out)
+    return res.stderr
+
+
+def build_host(force: bool = False) -> str:
+    """Compile the host extension if its source is newer than it; return its path."""
+    if not force and os.path.exists(HOST_OUT) and os.path.getmtime(HOST_SOURCE) <= os.path.getmtime(HOST_OUT):
+        return HOST_OUT
+    import torch
+    from torch.utils import cpp_extension
+
+    cuda_home = os.path.dirname(os.path.dirname(os.path.realpath(_nvcc())))
+    includes = [*cpp_extension.include_paths(), os.path.join(cuda_home, "include"), sysconfig.get_paths()["include"]]
+    lib_dir = os.path.join(os.path.dirname(torch.__file__), "lib")
+    tmp = f"{HOST_OUT}.{os.getpid()}.tmp"
+    cmd = [
+        shutil.which("g++") or "g++", "-O2", "-std=c++17", "-shared", "-fPIC",
+        f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}",
+        *[f"-I{p}" for p in includes], "-o", tmp, HOST_SOURCE,
+        f"-L{lib_dir}", "-ltorch_python", "-ltorch", "-lc10", "-lc10_cuda", f"-Wl,-rpath,{lib_dir}",
+    ]  # fmt: skip
+    _run(cmd, tmp, HOST_OUT)
+    return HOST_OUT
+
+
 def build(force: bool = False, verbose: bool = False, extra_flags: list[str] | None = None) -> str:
-    """Compile the library if any source is newer than it; return the path of the shared object."""
+    """Compile the library and the host extension where a source is newer; return the path of the library."""
+    build_host(force)
     if not force and not needs_build():
         return OUT
     cmd = [_nvcc(), *NVCC_FLAGS, *(extra_flags or [])]
     if verbose:
         cmd += ["-Xptxas", "-v"]
-    tmp = f"{OUT}.{os.getpid()}.tmp"  # a reader never sees a half-written library
+    tmp = f"{OUT}.{os.getpid()}.tmp"
     cmd += ["-o", tmp, *[os.path.join(CSRC, s) for s in SOURCES]]
-    res = subprocess.run(cmd, capture_output=True, text=True)
-    if res.returncode != 0:
-        if os.path.exists(tmp):
-            os.remove(tmp)
-        raise RuntimeError(f"nvcc failed:\n{' '.join(cmd)}\n{res.stdout}\n{res.stderr}")
-    os.replace(tmp, OUT)
+    messages = _run(cmd, tmp, OUT)
     if verbose:
-        print(res.stderr, file=sys.stderr)
+        print(messages, file=sys.stderr)
     return OUT
 
 

@@ -964,6 +964,7 @@ int eo_adamw_step(int n, const int64_t* host_table, const eo_adamw_config* confi
   c.one_minus_beta2 = static_cast<float>(1.0 - cfg.beta2);
   c.eps = static_cast<float>(cfg.eps);
   c.l2 = cfg.decay_method == eo::kDecayL2 ? static_cast<float>(cfg.weight_decay) : 0.0f;
+  c.minus_zero = -0.0f;
   c.seed = cfg.seed;
   c.f = eo::AdamWFactors{};
   if (!device_factors)

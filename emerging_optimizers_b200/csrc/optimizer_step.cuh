@@ -167,6 +167,9 @@ __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
   return d;
 }
 __device__ __forceinline__ float2 both(float x) { return make_float2(x, x); }
+// a * b, rounded before anything is done with it: the assembler fuses a paired multiplication with a following addition, but not
+// a fused one whose addend it does not know.  minus_zero: -0, from a kernel parameter.
+__device__ __forceinline__ float2 product(float2 a, float2 b, float2 minus_zero) { return fma2(a, b, minus_zero); }
 
 // bf16 weights whose fp32 master is kept as bf16 plus a signed 16-bit remainder: master bits = (bf16 bits << 16) +
 // remainder.  Written back as the nearest bf16 (halves away from zero, so that the remainder fits 16 bits); a NaN
@@ -396,7 +399,7 @@ struct AdamWFactors {
 };
 
 struct AdamWScalars {
-  float beta1, one_minus_beta1, beta2, one_minus_beta2, eps, l2;
+  float beta1, one_minus_beta1, beta2, one_minus_beta2, eps, l2, minus_zero;
   uint32_t seed;
   AdamWFactors f;             // used when dev_factors is nullptr
   const AdamWFactors* dev_factors;  // per tensor of this launch, from adamw_factors_kernel
@@ -459,26 +462,26 @@ __device__ __forceinline__ void adamw_update(float2 (&p)[4], const float2 (&g_in
                                              const AdamWScalars& c, const AdamWFactors& f, float grad_scale) {
   const float2 scale = both(grad_scale), b1 = both(c.beta1), ob1 = both(c.one_minus_beta1), b2 = both(c.beta2);
   const float2 ob2 = both(c.one_minus_beta2), l2 = both(c.l2), eps = both(-c.eps), decay = both(f.decay);
-  const float2 size = both(-f.step_size), inv = both(f.inv_root_bc2 * 0x1p-12f);
+  const float2 size = both(-f.step_size), inv = both(f.inv_root_bc2 * 0x1p-12f), mz = both(c.minus_zero);
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
-    float2 g = mul2(g_in[k], scale);
-    if (c.l2 != 0.0f) g = add2(g, mul2(p[k], l2));
-    m[k] = add2(mul2(m[k], b1), mul2(g, ob1));
-    v[k] = add2(mul2(v[k], b2), mul2(mul2(g, g), ob2));
+    float2 g = product(g_in[k], scale, mz);
+    if (c.l2 != 0.0f) g = add2(g, product(p[k], l2, mz));
+    m[k] = add2(product(m[k], b1, mz), product(g, ob1, mz));
+    v[k] = add2(product(v[k], b2, mz), product(product(g, g, mz), ob2, mz));
     float2 nv = mul2(v[k], both(-0x1p24f));
     nv.x = at_least(nv.x, -3.4028234664e38f);
     nv.y = at_least(nv.y, -3.4028234664e38f);
     const float2 above_zero = add2(nv, both(-0x1p-126f));
     const float2 y = make_float2(rsqrt_approx(-above_zero.x), rsqrt_approx(-above_zero.y));
-    float2 nroot = mul2(nv, y);
+    float2 nroot = product(nv, y, mz);
     nroot = fma2(fma2(nroot, nroot, nv), mul2(y, both(0.5f)), nroot);
-    const float2 nd = add2(mul2(nroot, inv), eps);
+    const float2 nd = add2(product(nroot, inv, mz), eps);
     float2 z = make_float2(rcp_approx(-nd.x), rcp_approx(-nd.y));
     z = fma2(z, fma2(nd, z, both(1.0f)), z);
-    float2 q = mul2(m[k], z);
+    float2 q = product(m[k], z, mz);
     q = fma2(fma2(nd, q, m[k]), z, q);
-    p[k] = add2(mul2(p[k], decay), mul2(q, size));
+    p[k] = add2(product(p[k], decay, mz), product(q, size, mz));
   }
 }
 

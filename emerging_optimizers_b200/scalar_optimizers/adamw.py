@@ -20,13 +20,11 @@ from emerging_optimizers_b200.scalar_optimizers.quantization import (
     exponent_count,
     quantize_blockwise,
 )
-from emerging_optimizers_b200.utils import tensor_lists
 
 
 __all__ = ["AdamW", "adamw_step", "adamw_step_8bit"]
 
 _FLOATS = (torch.float32, torch.bfloat16)
-_F32, _U8, _I16, _I64 = (torch.float32,), (torch.uint8,), (torch.int16,), (torch.int64,)
 _MASK32 = (1 << 32) - 1
 
 
@@ -50,58 +48,24 @@ def _device_scalar(value: Any, name: str, device: int, dtype: torch.dtype) -> to
 
 
 def _step(
-    params, grads, m, v, m_exponents, v_exponents, remainders, *, state_bits, lr, betas, eps, weight_decay, step,
+    params, grads, m, v, m_exponents, v_exponents, remainders, *, lr, betas, eps, weight_decay, step,
     weight_decay_method, grad_scale, seed=0, first_index=0,
 ) -> None:  # fmt: skip
     _check_hyperparameters(lr, betas, eps, weight_decay, weight_decay_method)
+    if not (0 <= seed <= _MASK32):
+        raise ValueError(f"seed must be in [0, 2^32), got {seed}")
     params = list(params)
-    n = len(params)
-    if n == 0:
+    if not params:
         return
-    device = tensor_lists.common_device(params, "params")
-    column = tensor_lists.addresses
-    p_ptrs = column(params, "params", device, _FLOATS)
-    numels = list(map(torch.Tensor.numel, params))
-    columns = [p_ptrs, column(grads, "grads", device, _FLOATS, numels)]
-    zeros = [0] * n
-    if state_bits == 8:
-        counts = [exponent_count(k) for k in numels]
-        columns += [
-            column(m, "exp_avgs", device, _U8, numels),
-            column(v, "exp_avg_sqs", device, _U8, numels),
-            column(m_exponents, "exp_avg_exponents", device, _U8, counts),
-            column(v_exponents, "exp_avg_sq_exponents", device, _U8, counts),
-        ]
-    else:
-        columns += [column(m, "exp_avgs", device, _F32, numels), column(v, "exp_avg_sqs", device, _F32, numels), zeros, zeros]
-    kinds = [
-        (p.dtype is torch.bfloat16) + 2 * (g.dtype is torch.bfloat16) for p, g in zip(params, grads)
-    ]  # fmt: skip
-    if remainders is None:
-        columns.append(zeros)
-    else:
-        if any(not k & _native.KIND_PARAM_BF16 for k in kinds):
-            raise TypeError("remainders go with bf16 parameters only")
-        columns.append(column(remainders, "remainders", device, _I16, numels))
-        kinds = [k | _native.KIND_REMAINDER for k in kinds]
-    written = {"params": columns[0], "exp_avgs": columns[2], "exp_avg_sqs": columns[3]}
-    if state_bits == 8:
-        written |= {"exp_avg_exponents": columns[4], "exp_avg_sq_exponents": columns[5]}
-    if remainders is not None:
-        written["remainders"] = columns[6]
-    tensor_lists.require_distinct(numels, **written)
-
-    if isinstance(step, int):
-        if step < 1:
-            raise ValueError(f"step counts from 1, got {step}")
-        if torch.cuda.is_current_stream_capturing():
-            raise RuntimeError("a step number given as an int would be frozen into the captured graph: pass an int64 device tensor")
-        columns.append(zeros)
-    else:
-        steps = [step] * n if torch.is_tensor(step) else list(step)
-        columns.append(column(steps, "step", device, _I64, [1] * n))
-        step = 0
-    columns += [numels, kinds]
+    on_host = isinstance(step, int)
+    if on_host and step < 1:
+        raise ValueError(f"step counts from 1, got {step}")
+    host = _native.host()
+    device, table, kinds = host.adamw_table(
+        params, grads, m, v, m_exponents, v_exponents, remainders, None if on_host else step
+    )
+    if on_host and host.stream(device)[2]:
+        raise RuntimeError("a step number given as an int would be frozen into the captured graph: pass an int64 device tensor")
     lr_tensor = None
     if torch.is_tensor(lr):
         if lr.is_cuda:
@@ -110,13 +74,12 @@ def _step(
             lr = float(lr)
     if grad_scale is not None:
         _device_scalar(grad_scale, "grad_scale", device, torch.float32)
-    if not (0 <= seed <= _MASK32):
-        raise ValueError(f"seed must be in [0, 2^32), got {seed}")
     _native.adamw_step(
-        device, columns, lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, method=weight_decay_method, step=step,
-        state_bits=state_bits, seed=seed, first_index=first_index, lr_tensor=lr_tensor, grad_scale=grad_scale,
+        device, len(params), table, kinds, lr=lr, betas=betas, eps=eps, weight_decay=weight_decay,
+        method=weight_decay_method, step=step if on_host else 0, on_device=not on_host or lr_tensor is not None,
+        state_bits=32 if m_exponents is None else 8, seed=seed, first_index=first_index, lr_tensor=lr_tensor,
+        grad_scale=grad_scale,
     )  # fmt: skip
-    tensor_lists.mark_written(params)
 
 
 @torch.no_grad()
@@ -152,7 +115,7 @@ def adamw_step(
             step and loses updates below half its last place.
     """
     _step(
-        params, grads, exp_avgs, exp_avg_sqs, None, None, remainders, state_bits=32, lr=lr, betas=betas, eps=eps,
+        params, grads, exp_avgs, exp_avg_sqs, None, None, remainders, lr=lr, betas=betas, eps=eps,
         weight_decay=weight_decay, step=step, weight_decay_method=weight_decay_method, grad_scale=grad_scale,
     )  # fmt: skip
 
@@ -184,7 +147,7 @@ def adamw_step_8bit(
     nearest, a moving average in 8 bits stands still as soon as a step moves it by less than half a unit.
     """
     _step(
-        params, grads, exp_avgs, exp_avg_sqs, exp_avg_exponents, exp_avg_sq_exponents, remainders, state_bits=8, lr=lr,
+        params, grads, exp_avgs, exp_avg_sqs, exp_avg_exponents, exp_avg_sq_exponents, remainders, lr=lr,
         betas=betas, eps=eps, weight_decay=weight_decay, step=step, weight_decay_method=weight_decay_method,
         grad_scale=grad_scale, seed=seed,
     )  # fmt: skip
@@ -297,44 +260,45 @@ class AdamW(optim.Optimizer):
             raise ValueError("closure is not supported")
         first_index = 0
         for group in self.param_groups:
-            # one call per device and step number; with device counters one per device
-            calls: dict[tuple, list[torch.Tensor]] = {}
-            for p in group["params"]:
-                grad = p.grad
-                if grad is None:
-                    continue
-                if grad.is_sparse:
-                    raise RuntimeError("AdamW does not support sparse gradients")
-                state = self.state[p]
-                if not state:
+            params = [p for p in group["params"] if p.grad is not None]
+            if any(p.grad.is_sparse for p in params):
+                raise RuntimeError("AdamW does not support sparse gradients")
+            for p in params:
+                if not self.state[p]:
                     if p.is_cuda and torch.cuda.is_current_stream_capturing():
                         raise RuntimeError("run a step before capturing one: the state must exist when the capture begins")
-                    state.update(self._new_state(p))
-                step = 0 if self.capturable else state["step"] + 1
-                calls.setdefault((p.get_device(), step, self._has_remainder(p)), []).append(p)
-            for (_, step, remainder), params in calls.items():
-                self._call(group, params, step, remainder, grad_scale, first_index)
-                first_index += len(params)
+                    self.state[p] = self._new_state(p)
+            # one call per device, kind of parameter and step number (with device counters: whatever the number)
+            keys = [
+                (p.get_device(), p.dtype, 0 if self.capturable else self.state[p]["step"] + 1) for p in params
+            ]  # fmt: skip
+            for key in dict.fromkeys(keys):
+                chosen = params if keys.count(key) == len(keys) else [p for p, k in zip(params, keys) if k == key]
+                self._call(group, chosen, key[2], grad_scale, first_index)
+                first_index += len(chosen)
         return None
 
-    def _call(self, group, params, step, remainder, grad_scale, first_index) -> None:  # type: ignore[no-untyped-def]
+    def _call(self, group, params, step, grad_scale, first_index) -> None:  # type: ignore[no-untyped-def]
         states = [self.state[p] for p in params]
-        orders = [None if p.is_contiguous() else _memory_order(p) for p in params]
-        plain = not any(orders)
+        grads = [p.grad for p in params]
+        plain = all(map(torch.Tensor.is_contiguous, params))
+        orders = [None] * len(params) if plain else [_memory_order(p) for p in params]
+        if not plain or not all(map(torch.Tensor.is_contiguous, grads)):
+            grads = [_flat(g, o) for g, o in zip(grads, orders)]
 
         def column(name):  # type: ignore[no-untyped-def]
             ts = [s[name] for s in states]
             return ts if plain else [_flat(t, o) for t, o in zip(ts, orders)]
 
-        grads = [p.grad for p in params]
-        grads = [g if o is None and g.is_contiguous() else _flat(g, o) for g, o in zip(grads, orders)]
         if self.capturable:
             step = [s["step"] for s in states]
             torch._foreach_add_(step, 1)
-        exponents = [[s[name] for s in states] for name in ("exp_avg_exponents", "exp_avg_sq_exponents")] if self.state_bits == 8 else (None, None)
+        exponents = [None, None]
+        if self.state_bits == 8:
+            exponents = [[s[name] for s in states] for name in ("exp_avg_exponents", "exp_avg_sq_exponents")]
         _step(
             params if plain else [_flat(p, o) for p, o in zip(params, orders)], grads, column("exp_avg"), column("exp_avg_sq"),
-            *exponents, column("remainder") if remainder else None, state_bits=self.state_bits, lr=group["lr"],
+            *exponents, column("remainder") if self._has_remainder(params[0]) else None, lr=group["lr"],
             betas=group["betas"], eps=group["eps"], weight_decay=group["weight_decay"], step=step,
             weight_decay_method=self.weight_decay_method, grad_scale=grad_scale, seed=self.seed, first_index=first_index,
         )  # fmt: skip

@@ -11,7 +11,6 @@ from __future__ import annotations
 import torch
 
 from emerging_optimizers_b200 import _native
-from emerging_optimizers_b200.utils import tensor_lists
 
 
 __all__ = ["dequantize_blockwise", "quantize_blockwise"]
@@ -27,7 +26,7 @@ def exponent_count(numel: int) -> int:
 @torch.no_grad()
 def quantize_blockwise(
     x: torch.Tensor, *, signed: bool, seed: int | None = None
-) -> tuple[torch.Tensor, torch.Tensor]:  # fmt: skip
+) -> tuple[torch.Tensor, torch.Tensor]:
     """Codes (uint8, the shape of ``x``) and exponent bytes (uint8, one per 256 elements) of a contiguous fp32 or bf16
     CUDA tensor.
 
@@ -35,7 +34,10 @@ def quantize_blockwise(
     part cut off, with random bits that depend on the seed and the element's place only.
     """
     _native.require_cuda(x, "x")
-    tensor_lists.addresses([x], "x", x.get_device(), _VALUES)
+    if x.dtype not in _VALUES:
+        raise TypeError(f"x must be torch.float32 or torch.bfloat16, got {x.dtype}")
+    if not x.is_contiguous():
+        raise ValueError(f"x is not contiguous (shape {tuple(x.shape)}, strides {x.stride()})")
     if seed is not None and not 0 <= seed < 1 << 32:
         raise ValueError(f"seed must be in [0, 2^32), got {seed}")
     codes = torch.empty(x.shape, dtype=torch.uint8, device=x.device)
@@ -53,8 +55,12 @@ def dequantize_blockwise(
     _native.require_cuda(codes, "codes")
     if dtype not in _VALUES:
         raise TypeError(f"dtype must be torch.float32 or torch.bfloat16, got {dtype}")
-    tensor_lists.addresses([codes], "codes", codes.get_device(), [torch.uint8])
-    tensor_lists.addresses([exponents], "exponents", codes.get_device(), [torch.uint8], [exponent_count(codes.numel())])
+    if codes.dtype != torch.uint8 or exponents.dtype != torch.uint8:
+        raise TypeError(f"codes and exponents must be torch.uint8, got {codes.dtype} and {exponents.dtype}")
+    if exponents.device != codes.device or exponents.numel() != exponent_count(codes.numel()):
+        raise ValueError(f"exponents must be {exponent_count(codes.numel())} bytes on {codes.device}")
+    if not (codes.is_contiguous() and exponents.is_contiguous()):
+        raise ValueError("codes and exponents must be contiguous")
     out = torch.empty(codes.shape, dtype=dtype, device=codes.device)
     _native.dequantize_blockwise(codes, exponents, signed, out)
     return out

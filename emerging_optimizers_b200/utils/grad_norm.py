@@ -13,29 +13,17 @@ from typing import Iterable, Sequence
 import torch
 
 from emerging_optimizers_b200 import _native
-from emerging_optimizers_b200.utils import tensor_lists
 
 
 __all__ = ["clip_coefficient", "clip_grad_norm_", "clip_grads_", "global_grad_norm"]
 
-_DTYPES = (torch.float32, torch.bfloat16)
-
 
 def _norm(grads: Sequence[torch.Tensor], max_norm: float, in_place: bool) -> torch.Tensor:
-    grads = list(grads)
-    if not grads:
-        raise ValueError("no gradients given")
     if not max_norm >= 0.0:
         raise ValueError(f"max_norm must not be negative, got {max_norm}")
-    device = tensor_lists.common_device(grads, "grads")
-    ptrs = tensor_lists.addresses(grads, "grads", device, _DTYPES)
-    numels = list(map(torch.Tensor.numel, grads))
-    if in_place:
-        tensor_lists.require_distinct(numels, grads=ptrs)
-    out = _native.grad_norm(device, [ptrs, numels, [g.dtype is torch.bfloat16 for g in grads]], max_norm, in_place)
-    if in_place:
-        tensor_lists.mark_written(grads)
-    return out
+    grads = list(grads)
+    device, table, types = _native.host().grads_table(grads, in_place)
+    return _native.grad_norm(device, grads[0].device, len(grads), table, types, max_norm, in_place)
 
 
 @torch.no_grad()
@@ -51,8 +39,8 @@ def clip_coefficient(grads: Sequence[torch.Tensor], max_norm: float) -> tuple[to
 
     Pass the coefficient to ``AdamW.step(grad_scale=...)``.  A norm that is NaN gives a coefficient that is NaN.
     """
-    out = _norm(grads, max_norm, False)
-    return out[0], out[1]
+    norm, coefficient = _norm(grads, max_norm, False).unbind()
+    return norm, coefficient
 
 
 @torch.no_grad()

@@ -86,6 +86,28 @@ def test_adamw_step_against_float64(method, p_dtype, g_dtype, scaled):
         assert np.all(np.abs(_np64(p) - p64) <= (16 * ULP * pm) * (1 + 2.0**-8) + last)
 
 
+@pytest.mark.parametrize("method", ["decoupled", "l2"])
+@pytest.mark.parametrize("steps", [(1, 2, 3), (1000, 100000)])
+def test_adamw_step_gives_the_bits_of_single_operations(method, steps):
+    """Parameters and moments are bit for bit what torch's elementary fp32 operations leave, each rounded once: no
+    contraction, the root and the quotient to nearest.  2^23 elements: about every mantissa under the root."""
+    (p,), (g,), (m,), (v,) = _inputs([1 << 23])
+    m *= torch.exp(4 * _randn(1 << 23, 91))
+    v *= torch.exp(8 * _randn(1 << 23, 92))
+    p0, m0, v0 = p.clone(), m.clone(), v.clone()
+    lr, (b1, b2), eps, wd = HYPER["lr"], HYPER["betas"], HYPER["eps"], HYPER["weight_decay"]
+    for step in steps:
+        adamw_step([p], [g], [m], [v], **HYPER, step=step, weight_decay_method=method, grad_scale=torch.tensor(0.7, device="cuda"))
+        x = g * torch.tensor(0.7, device="cuda")
+        if method == "l2":
+            x = x + p0 * wd
+        p0 = p0 * ref.decay_factor(method, lr, wd)
+        m0 = m0 * b1 + x * (1 - b1)
+        v0 = v0 * b2 + (x * x) * (1 - b2)
+        p0 = p0 - (m0 / (v0.sqrt() * (1 / (1 - b2**step) ** 0.5) + eps)) * (lr / (1 - b1**step))
+        assert _same(m, m0) and _same(v, v0) and _same(p, p0)
+
+
 @pytest.mark.parametrize("off", [(1, 0, 0, 0), (0, 1, 0, 0), (0, 0, 3, 0), (0, 0, 0, 5), (1, 2, 3, 4)])
 @pytest.mark.parametrize("dtype", [F32, BF16])
 def test_adamw_step_at_any_alignment_gives_the_same_bits(off, dtype):
@@ -455,7 +477,7 @@ def test_optimizer_matches_torch_adamw():
             s.step()
     for p, q in zip(a, b):
         # an update is at most lr (0.01) times a few; both sides are within some 20 roundings of the exact one
-        assert torch.allclose(p, q, rtol=0, atol=6 * 1e-2 * 3 * 20 * ULP + 6 * 2 * ULP * float(q.abs().max()))
+        assert torch.allclose(p, q, rtol=0, atol=6 * 1e-2 * 3 * 20 * ULP + 6 * 2 * ULP * float(q.detach().abs().max()))
         assert ours.state[p]["step"] == int(theirs.state[q]["step"])
     c = _model_params()
     third = AdamW([{"params": c[:2]}, {"params": c[2:]}])

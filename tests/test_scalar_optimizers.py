@@ -6,6 +6,7 @@ import pytest
 import torch
 
 from emerging_optimizers_b200 import _native, registry, utils
+from emerging_optimizers_b200 import build as eo_build
 from emerging_optimizers_b200.scalar_optimizers import (
     AdamW,
     adamw_step,
@@ -14,6 +15,11 @@ from emerging_optimizers_b200.scalar_optimizers import (
     quantize_blockwise,
 )
 from tests import _scalar_ref as ref
+
+
+@pytest.fixture(scope="module", autouse=True)
+def built():
+    eo_build.build()
 
 
 def _p(*shape, dtype=torch.float32):
