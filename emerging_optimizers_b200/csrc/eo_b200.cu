@@ -1075,12 +1075,19 @@ int eo_quantize_blockwise(const void* x, int dtype, int64_t numel, int is_signed
   const uint32_t key = eo::rounding_key(seed, 0, 0);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const unsigned g = static_cast<unsigned>(grid);
-#define EO_QUANTIZE(T, S)                                                                                             \
-  eo::quantize_kernel<T, S><<<g, eo::kOptThreads, 0, s>>>(static_cast<const T*>(x), numel, vec, random, key, codes, exponents)
+#define EO_QUANTIZE(T, S)                                                                                                 \
+  do {                                                                                                                    \
+    if (random)                                                                                                           \
+      eo::quantize_kernel<T, S, true><<<g, eo::kOptThreads, 0, s>>>(static_cast<const T*>(x), numel, vec, key, codes, exponents);  \
+    else                                                                                                                  \
+      eo::quantize_kernel<T, S, false><<<g, eo::kOptThreads, 0, s>>>(static_cast<const T*>(x), numel, vec, key, codes, exponents); \
+  } while (0)
   if (dtype == EO_F32) {
-    if (is_signed) EO_QUANTIZE(float, true); else EO_QUANTIZE(float, false);
+    if (is_signed) EO_QUANTIZE(float, true);
+    else EO_QUANTIZE(float, false);
   } else {
-    if (is_signed) EO_QUANTIZE(__nv_bfloat16, true); else EO_QUANTIZE(__nv_bfloat16, false);
+    if (is_signed) EO_QUANTIZE(__nv_bfloat16, true);
+    else EO_QUANTIZE(__nv_bfloat16, false);
   }
 #undef EO_QUANTIZE
   EO_CUDA(cudaGetLastError());

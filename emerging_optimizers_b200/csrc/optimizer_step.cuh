@@ -213,9 +213,6 @@ __device__ __forceinline__ void split_masters(const float2 (&x)[4], Run<__nv_bfl
 // What this costs decides the speed of the 8-bit step, and the integer pipe has half the rate of the floating-point one:
 // everything an element needs is a multiplication or an add, except the byte moves.  What is not finite is looked for
 // once per block, in the maximum that the exponent needs anyway, and dealt with off the common path.
-__device__ __forceinline__ float power_of_two(int e) {  // e in -149 .. 127
-  return __uint_as_float(e >= -126 ? static_cast<uint32_t>(e + 127) << 23 : 1u << (e + 149));
-}
 __device__ __forceinline__ float max3_nan(float a, float b, float c) {
   float d;
   asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
@@ -232,7 +229,7 @@ struct Code8 {
   static __device__ __forceinline__ void decode(const Run<uint8_t>& codes, uint32_t exponent, float2 (&out)[4]) {
     if constexpr (kSigned) {
       // The bits are those of e4m3 (sign, 4 exponent, 3 mantissa bits, 0x7f NaN), 2^7 times as large.
-      const float2 scale = both(power_of_two(static_cast<int>(exponent) - 134));
+      const float2 scale = both(__uint_as_float(exponent << 23) * 0x1p-7f);
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         uint32_t h2;
@@ -241,7 +238,7 @@ struct Code8 {
         out[k] = mul2(__half22float2(*reinterpret_cast<const __half2*>(&h2)), scale);
       }
     } else {
-      const float2 scale = both(power_of_two(static_cast<int>(exponent) - 127)), lift = both(up());
+      const float2 scale = both(__uint_as_float(exponent << 23)), lift = both(up());
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         const uint32_t w = codes.w[k / 2];
@@ -250,15 +247,13 @@ struct Code8 {
         const uint32_t b = __byte_perm(w, 0, 0x4044 | (2 * (k % 2) + 1) << 8) * 16u;
         out[k] = mul2(mul2(make_float2(__uint_as_float(a), __uint_as_float(b)), lift), scale);
       }
+      const uint32_t nans = ((~codes.w[0] - 0x01010101u) & codes.w[0]) | ((~codes.w[1] - 0x01010101u) & codes.w[1]);
+      if (nans & 0x80808080u) {  // a byte is 0xff
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const uint32_t w = codes.w[j];
-        if ((~w - 0x01010101u) & w & 0x80808080u) {  // a byte is 0xff
-#pragma unroll
-          for (int k = 0; k < 2; ++k) {
-            if (((w >> (16 * k)) & 0xffu) == kNan) out[2 * j + k].x = __uint_as_float(0x7fc00000u);
-            if (((w >> (16 * k + 8)) & 0xffu) == kNan) out[2 * j + k].y = __uint_as_float(0x7fc00000u);
-          }
+        for (int k = 0; k < 4; ++k) {
+          const uint32_t two = codes.w[k / 2] >> (16 * (k % 2));
+          if ((two & 0xffu) == kNan) out[k].x = __uint_as_float(0x7fc00000u);
+          if (((two >> 8) & 0xffu) == kNan) out[k].y = __uint_as_float(0x7fc00000u);
         }
       }
     }
@@ -282,13 +277,12 @@ struct Code8 {
     return (kSigned ? (b & 0x7fffffffu) : b) < 0x7f800000u;
   }
 
-  // Exponent byte and codes of a block; r[k]: sixteen random bits for each element (unused when to nearest).
-  static __device__ __forceinline__ uint32_t quantize(const float2 (&in)[4], bool random, const uint32_t (&r)[8],
-                                                      Run<uint8_t>& codes) {
+  // Exponent byte and codes of a block; d16[k]: 16 d of each element.
+  static __device__ __forceinline__ uint32_t quantize(const float2 (&in)[4], const uint32_t (&d16)[8], Run<uint8_t>& codes) {
     const float x[8] = {in[0].x, in[0].y, in[1].x, in[1].y, in[2].x, in[2].y, in[3].x, in[3].y};
     uint32_t top = block_top(x);
-    const bool special = top >= 0x7f800000u;
-    if (special) {
+    const bool rare = top >= 0x7f000000u;  // 2^127 and beyond, infinity, NaN; unsigned: a negative number
+    if (rare) {
       uint32_t mine = 0;
 #pragma unroll
       for (int k = 0; k < 8; ++k)
@@ -296,18 +290,29 @@ struct Code8 {
       top = __reduce_max_sync(0xffffffffu, mine);
     }
     const uint32_t e = max(top >> 23, 1u);
-    const float2 inv = both(power_of_two(127 - static_cast<int>(e))), lower = both(down());
-    // 16 (bits + d) has the code in its top byte; the sign, if any, is shifted out.  The two constants make 16 d.
-    const uint32_t mul = random && e < 254u ? 256u : 0u, add = e >= 254u ? 0u : random ? 128u : 0x800000u;
+    // 2^(127 - e); subnormal for e = 254
+    const float2 inv = both(__uint_as_float(max((254u - e) << 23, 0x00400000u))), lower = both(down());
     uint32_t t[8];
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
+      // 16 (bits + d) has the code in its top byte; the sign, if any, is shifted out
       const float2 y = mul2(mul2(in[k], inv), lower);
-      t[2 * k] = __float_as_uint(y.x) * 16u + (r[2 * k] * mul + add);
-      t[2 * k + 1] = __float_as_uint(y.y) * 16u + (r[2 * k + 1] * mul + add);
+      t[2 * k] = __float_as_uint(y.x) * 16u + d16[2 * k];
+      t[2 * k + 1] = __float_as_uint(y.y) * 16u + d16[2 * k + 1];
       if constexpr (!kSigned) {
         if (in[k].x > 0.0f) t[2 * k] = max(t[2 * k], 1u << 24);
         if (in[k].y > 0.0f) t[2 * k + 1] = max(t[2 * k + 1], 1u << 24);
+      }
+    }
+    if (rare) {
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const float v = k % 2 == 0 ? in[k / 2].x : in[k / 2].y;
+        if (e == 254u) {  // towards zero: without d
+          t[k] -= d16[k];
+          if (!kSigned && v > 0.0f) t[k] = max(__float_as_uint(__fmul_rn(__fmul_rn(v, inv.x), lower.x)) * 16u, 1u << 24);
+        }
+        if (!is_kept(v)) t[k] = (!kSigned && __float_as_uint(v) == 0x80000000u) ? 0u : kNan << 24;  // -0 is kept as 0
       }
     }
 #pragma unroll
@@ -318,14 +323,6 @@ struct Code8 {
             __byte_perm(__float_as_uint(x[4 * j]), __float_as_uint(x[4 * j + 1]), 0x0073),
             __byte_perm(__float_as_uint(x[4 * j + 2]), __float_as_uint(x[4 * j + 3]), 0x0073), 0x5410);
         w = (w & 0x7f7f7f7fu) | (signs & 0x80808080u);
-      }
-      if (special) {
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const uint32_t b = __float_as_uint(x[4 * j + k]);
-          if (!is_kept(x[4 * j + k]))
-            w = (w & ~(0xffu << (8 * k))) | ((!kSigned && b == 0x80000000u ? 0u : kNan | (kSigned ? (b >> 24) & 0x80u : 0u)) << (8 * k));
-        }
       }
       codes.w[j] = w;
     }
@@ -342,18 +339,19 @@ __host__ __device__ __forceinline__ uint32_t mix32(uint32_t x) {
 __host__ __device__ __forceinline__ uint32_t rounding_key(uint32_t seed, uint32_t tensor, uint32_t step) {
   return mix32(mix32(mix32(seed) ^ tensor) ^ step);
 }
-// mix32(key ^ element) of a lane's eight elements, halves apart.  The elements of a lane differ in bits below 16 only, which
-// the first step of the mixer leaves alone, so that step is done once.
+// 16 d = 256 r + 128 of a lane's eight elements, r the low (first moments) and the high half (second moments) of
+// mix32(key ^ element); `first`: the lane's first element.  Elements of a lane differ in bits below 16 only, which the first
+// step of the mixer leaves alone, so that step is done once; its last one is the exclusive or of the halves.
 template <bool kVec>
-__device__ __forceinline__ void random_halves(uint32_t key, uint32_t first, uint32_t (&low)[8], uint32_t (&high)[8]) {
-  first ^= key;  // `first`: the lane's first element
+__device__ __forceinline__ void random_dither(uint32_t key, uint32_t first, uint32_t (&low)[8], uint32_t (&high)[8]) {
+  first ^= key;
   first ^= first >> 16;
 #pragma unroll
   for (int k = 0; k < 8; ++k) {
     uint32_t x = (first ^ static_cast<uint32_t>(kVec ? k : 32 * k)) * 0x85ebca6bu;
     x = (x ^ (x >> 13)) * 0xc2b2ae35u;
-    high[k] = x >> 16;
-    low[k] = (x ^ high[k]) & 0xffffu;
+    high[k] = __byte_perm(x, 0x80u, 0x5324);                // 0, the high half, 0x80
+    low[k] = __byte_perm(x, 0x80u, 0x5105) ^ high[k];       // 0, the halves' exclusive or, 0x80
   }
 }
 
@@ -513,9 +511,9 @@ struct AdamWRun {
     if constexpr (kRemainder) split_masters(xp, p, r); else p.pack(xp);
     if constexpr (k8) {
       uint32_t low[8], high[8];
-      random_halves<kVec>(key, first, low, high);
-      me = Code8<true>::quantize(xm, true, low, m);
-      ve = Code8<false>::quantize(xv, true, high, v);
+      random_dither<kVec>(key, first, low, high);
+      me = Code8<true>::quantize(xm, low, m);
+      ve = Code8<false>::quantize(xv, high, v);
     } else {
       m.pack(xm);
       v.pack(xv);
@@ -524,19 +522,18 @@ struct AdamWRun {
 };
 
 // Addresses of a lane's elements in whole, aligned runs; they move on by one trip.
-template <typename P, typename G, bool kRemainder, bool k8>
+template <typename P, typename G, bool kRemainder>
 struct AdamWCursor {
-  using Data = AdamWRun<P, G, kRemainder, k8>;
-  using Moment = typename Data::Moment;
+  using Data = AdamWRun<P, G, kRemainder, false>;
   P* p;
   const G* g;
-  Moment *m, *v;
+  float *m, *v;
   int16_t* r;
   __device__ __forceinline__ AdamWCursor(const AdamWEntry& t, long long at, int lane)
       : p(static_cast<P*>(t.p) + at + 8 * lane),
         g(static_cast<const G*>(t.g) + at + 8 * lane),
-        m(static_cast<Moment*>(t.m) + at + 8 * lane),
-        v(static_cast<Moment*>(t.v) + at + 8 * lane),
+        m(static_cast<float*>(t.m) + at + 8 * lane),
+        v(static_cast<float*>(t.v) + at + 8 * lane),
         r(t.r + at + 8 * lane) {}
   __device__ __forceinline__ void get(Data& d) const {
     d.g.get(g);
@@ -565,27 +562,41 @@ template <typename P, typename G, bool kRemainder>
 struct AdamWRing {
   static constexpr int kP = 0, kG = kP + kOptRun * sizeof(P), kM = kG + kOptRun * sizeof(G), kV = kM + kOptRun,
                        kR = kV + kOptRun, kBytes = kR + (kRemainder ? 2 * kOptRun : 0);
-  static constexpr int kCtaBytes = kBytes * kRingStages * (kOptThreads / 32);
+  static constexpr int kWarpBytes = kBytes * kRingStages, kCtaBytes = kWarpBytes * (kOptThreads / 32);
+  static constexpr int kAhead = (kRingStages - 1) * kOptTrip;  // elements between the run fetched and the run worked on
+
+  // A lane's addresses in the run to be fetched: it copies other elements than it works on where its eight take 32 bytes.
+  const char *p, *g;
+  uint8_t *m, *v;
+  int16_t* r;
+  __device__ __forceinline__ AdamWRing(const AdamWEntry& t, long long at, int lane)
+      : p(reinterpret_cast<const char*>(static_cast<const P*>(t.p) + at) + 16 * lane),
+        g(reinterpret_cast<const char*>(static_cast<const G*>(t.g) + at) + 16 * lane),
+        m(static_cast<uint8_t*>(t.m) + at + 8 * lane),
+        v(static_cast<uint8_t*>(t.v) + at + 8 * lane),
+        r(t.r + at + 8 * lane) {}
 
   template <int kRunBytes>
-  static __device__ __forceinline__ void copy(uint32_t to, const void* run, int lane) {
-    constexpr int kPiece = kRunBytes >= 512 ? 16 : 8;
-    const char* from = static_cast<const char*>(run) + kPiece * lane;
-#pragma unroll
-    for (int at = 0; at < kRunBytes; at += 32 * kPiece) {
-      if constexpr (kPiece == 16)
-        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to + at + kPiece * lane), "l"(from + at) : "memory");
-      else
-        asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(to + at + kPiece * lane), "l"(from + at) : "memory");
+  static __device__ __forceinline__ void copy(uint32_t to, const void* from) {
+    if constexpr (kRunBytes == 256) {
+      asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(to), "l"(from) : "memory");
+    } else {
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
+      if constexpr (kRunBytes == 1024)
+        asm volatile("cp.async.cg.shared.global [%0+512], [%1+512], 16;" ::"r"(to), "l"(from) : "memory");
     }
   }
-  // `at`: first element of the run
-  static __device__ __forceinline__ void fetch(uint32_t stage, const AdamWEntry& t, long long at, int lane) {
-    copy<kOptRun * sizeof(P)>(stage + kP, static_cast<const P*>(t.p) + at, lane);
-    copy<kOptRun * sizeof(G)>(stage + kG, static_cast<const G*>(t.g) + at, lane);
-    copy<kOptRun>(stage + kM, static_cast<const uint8_t*>(t.m) + at, lane);
-    copy<kOptRun>(stage + kV, static_cast<const uint8_t*>(t.v) + at, lane);
-    if constexpr (kRemainder) copy<kOptRun * 2>(stage + kR, t.r + at, lane);
+  // stage: shared address of the stage, plus 8 lane
+  __device__ __forceinline__ void fetch(uint32_t stage, int lane) const {
+    copy<kOptRun * sizeof(P)>(stage + 8 * lane + kP, p);
+    copy<kOptRun * sizeof(G)>(stage + 8 * lane + kG, g);
+    copy<kOptRun>(stage + kM, m);
+    copy<kOptRun>(stage + kV, v);
+    if constexpr (kRemainder) copy<kOptRun * 2>(stage + 8 * lane + kR, r);
+  }
+  __device__ __forceinline__ void next() {
+    p += kOptTrip * sizeof(P), g += kOptTrip * sizeof(G), m += kOptTrip, v += kOptTrip;
+    if constexpr (kRemainder) r += kOptTrip;
   }
   static __device__ __forceinline__ void read(const char* stage, int lane, AdamWRun<P, G, kRemainder, true>& d) {
     d.p = reinterpret_cast<const Run<P>*>(stage + kP)[lane];
@@ -593,6 +604,13 @@ struct AdamWRing {
     d.m = reinterpret_cast<const Run<uint8_t>*>(stage + kM)[lane];
     d.v = reinterpret_cast<const Run<uint8_t>*>(stage + kV)[lane];
     if constexpr (kRemainder) d.r = reinterpret_cast<const Run<int16_t>*>(stage + kR)[lane];
+  }
+  // The run worked on lies kAhead elements before the one to be fetched.
+  __device__ __forceinline__ void put(const AdamWRun<P, G, kRemainder, true>& d, int lane) const {
+    d.p.put(reinterpret_cast<P*>(const_cast<char*>(p) + (sizeof(P) == 4 ? 16 * lane : 0)) - kAhead);
+    if constexpr (kRemainder) d.r.put(r - kAhead);
+    d.m.put(m - kAhead);
+    d.v.put(v - kAhead);
   }
 };
 
@@ -617,48 +635,54 @@ __global__ void __launch_bounds__(kOptThreads, 3)
   long long at = begin + warp * kOptRun;
   if (t.vec) {
     const int whole = end - at >= kOptRun ? static_cast<int>((end - at - kOptRun) / kOptTrip) + 1 : 0;
-    AdamWCursor<P, G, kRemainder, k8> cursor(t, at, lane);
     Data data;
     if constexpr (k8) {
       using Ring = AdamWRing<P, G, kRemainder>;
       extern __shared__ __align__(16) char ring_bytes[];
-      const char* ring = ring_bytes + warp * (Ring::kBytes * kRingStages);
-      const uint32_t ring_at = static_cast<uint32_t>(__cvta_generic_to_shared(ring));
+      const char* const stages = ring_bytes + warp * Ring::kWarpBytes;
+      const uint32_t stages_at = static_cast<uint32_t>(__cvta_generic_to_shared(stages)) + 8 * lane;
+      Ring ring(t, at, lane);
       uint8_t *me = t.me + at / kOptRun, *ve = t.ve + at / kOptRun;
-      uint32_t mes = 0, ves = 0;  // lane l: the exponents of the warp's run l from here
+      uint32_t mes = 0, ves = 0;  // lane l: the exponents of the warp's run l, of 32 at a time
+#pragma unroll
       for (int i = 0; i < kRingStages - 1; ++i) {
-        if (i < whole) Ring::fetch(ring_at + i * Ring::kBytes, t, at + static_cast<long long>(i) * kOptTrip, lane);
+        if (i < whole) ring.fetch(stages_at + i * Ring::kBytes, lane);
         asm volatile("cp.async.commit_group;" ::: "memory");
+        ring.next();
       }
-      int stage = 0;
-      for (int i = 0; i < whole; ++i, at += kOptTrip, cursor.next()) {
+      int stage = 0;  // byte offset of the run worked on
+      uint32_t first = static_cast<uint32_t>(at) + 8 * lane;
+      for (int i = 0; i < whole; ++i) {
         if ((i & 31) == 0 && i + lane < whole) {
           mes = me[(i + lane) * (kOptTrip / kOptRun)];
           ves = ve[(i + lane) * (kOptTrip / kOptRun)];
         }
         asm volatile("cp.async.wait_group %0;" ::"n"(kRingStages - 2) : "memory");
         __syncwarp();  // the run is there for all lanes, and all of them have read the one whose place is filled next
-        Ring::read(ring + stage * Ring::kBytes, lane, data);
-        if (i + kRingStages - 1 < whole)
-          Ring::fetch(ring_at + (stage == 0 ? kRingStages - 1 : stage - 1) * Ring::kBytes, t, at + (kRingStages - 1) * static_cast<long long>(kOptTrip), lane);
+        Ring::read(stages + stage, lane, data);
+        if (i + kRingStages - 1 < whole) ring.fetch(stages_at + (stage == 0 ? Ring::kWarpBytes : stage) - Ring::kBytes, lane);
         asm volatile("cp.async.commit_group;" ::: "memory");
-        stage = stage == kRingStages - 1 ? 0 : stage + 1;
+        stage = stage == Ring::kWarpBytes - Ring::kBytes ? 0 : stage + Ring::kBytes;
         data.me = __shfl_sync(0xffffffffu, mes, i & 31);
         data.ve = __shfl_sync(0xffffffffu, ves, i & 31);
-        data.template step<true>(c, f, grad_scale, key, static_cast<uint32_t>(at) + 8 * lane);
-        cursor.put(data);
+        data.template step<true>(c, f, grad_scale, key, first);
+        ring.put(data, lane);
         if (lane == 0) {
           me[i * (kOptTrip / kOptRun)] = static_cast<uint8_t>(data.me);
           ve[i * (kOptTrip / kOptRun)] = static_cast<uint8_t>(data.ve);
         }
+        ring.next();
+        first += kOptTrip;
       }
     } else {
-      for (int i = 0; i < whole; ++i, at += kOptTrip, cursor.next()) {
+      AdamWCursor<P, G, kRemainder> cursor(t, at, lane);
+      for (int i = 0; i < whole; ++i, cursor.next()) {
         cursor.get(data);
         data.template step<true>(c, f, grad_scale, key, 0u);
         cursor.put(data);
       }
     }
+    at += static_cast<long long>(whole) * kOptTrip;
   }
   for (; at < end; at += kOptTrip) {
     const long long left = end - at;
@@ -823,40 +847,48 @@ __global__ void __launch_bounds__(kOptThreads)
 constexpr int kQuantRuns = 4;
 constexpr int kQuantChunk = kQuantRuns * kOptTrip;  // elements of a CTA
 
-// `random`: stochastic rounding with `key`, else to nearest (halves away from zero).
-template <typename T, bool kSigned>
+// kRandom: rounded at random with `key`, else to nearest (halves away from zero).
+template <bool kVec, bool kSigned, bool kRandom, typename T>
+__device__ __forceinline__ uint32_t quantize_run(const Run<T>& run, uint32_t key, uint32_t first, Run<uint8_t>& out) {
+  float2 v[4];
+  run.unpack(v);
+  uint32_t low[8], high[8];
+  if constexpr (kRandom) {
+    random_dither<kVec>(key, first, low, high);
+  } else {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) low[k] = high[k] = 0x800000u;
+  }
+  return Code8<kSigned>::quantize(v, kSigned ? low : high, out);
+}
+template <typename T, bool kSigned, bool kRandom>
 __global__ void __launch_bounds__(kOptThreads)
-    quantize_kernel(const T* __restrict__ x, long long numel, int aligned, int random, uint32_t key,
-                    uint8_t* __restrict__ codes, uint8_t* __restrict__ exponents) {
+    quantize_kernel(const T* __restrict__ x, long long numel, int aligned, uint32_t key, uint8_t* __restrict__ codes,
+                    uint8_t* __restrict__ exponents) {
   const int lane = threadIdx.x & 31;
   const long long begin = static_cast<long long>(blockIdx.x) * kQuantChunk + (threadIdx.x >> 5) * kOptRun;
-  uint32_t low[8], high[8];
-  float2 v[4];
   Run<uint8_t> out;
   if (aligned && begin + (kQuantRuns - 1) * kOptTrip + kOptRun <= numel) {
     Run<T> run[kQuantRuns];
     const T* p = x + begin + 8 * lane;
+    uint8_t *to = codes + begin + 8 * lane, *e_to = exponents + begin / kOptRun;
     run[0].get(p);
     run[1].template get<kOptTrip>(p);
     run[2].template get<2 * kOptTrip>(p);
     run[3].template get<3 * kOptTrip>(p);
 #pragma unroll
     for (int i = 0; i < kQuantRuns; ++i) {
-      const long long at = begin + i * kOptTrip;
-      run[i].unpack(v);
-      random_halves<true>(key, static_cast<uint32_t>(at) + 8 * lane, low, high);
-      const uint32_t e = Code8<kSigned>::quantize(v, random != 0, kSigned ? low : high, out);
-      out.put(codes + at + 8 * lane);
-      if (lane == 0) exponents[at / kOptRun] = static_cast<uint8_t>(e);
+      const uint32_t first = static_cast<uint32_t>(begin) + i * kOptTrip + 8 * lane;
+      const uint32_t e = quantize_run<true, kSigned, kRandom>(run[i], key, first, out);
+      out.put(to + i * kOptTrip);
+      if (lane == 0) e_to[i * (kOptTrip / kOptRun)] = static_cast<uint8_t>(e);
     }
     return;
   }
   for (long long at = begin; at < numel && at < begin + kQuantChunk; at += kOptTrip) {
     Run<T> run;
     run.get_some(x + at, numel - at, lane);
-    run.unpack(v);
-    random_halves<false>(key, static_cast<uint32_t>(at) + lane, low, high);
-    const uint32_t e = Code8<kSigned>::quantize(v, random != 0, kSigned ? low : high, out);
+    const uint32_t e = quantize_run<false, kSigned, kRandom>(run, key, static_cast<uint32_t>(at) + lane, out);
     out.put_some(codes + at, numel - at, lane);
     if (lane == 0) exponents[at / kOptRun] = static_cast<uint8_t>(e);
   }
