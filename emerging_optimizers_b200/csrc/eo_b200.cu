@@ -1055,7 +1055,19 @@ int eo_grad_norm(int n, const int64_t* host_table, float max_norm, int in_place,
       };
       if (int rc = over_tables<eo::GradEntry>(n, fill, launch)) return rc;
     }
-    if (pass == 0) eo::grad_norm_final_kernel<<<1, eo::kEwThreads, 0, s>>>(partials, used, max_norm, out);
+    if (pass == 0) {
+      cudaLaunchAttribute early{};
+      early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+      early.val.programmaticStreamSerializationAllowed = 1;
+      cudaLaunchConfig_t config{};
+      config.gridDim = 1;
+      config.blockDim = eo::kNormThreads;
+      config.stream = s;
+      config.attrs = &early;
+      config.numAttrs = 1;
+      EO_CUDA(cudaLaunchKernelEx(&config, eo::grad_norm_final_kernel, static_cast<const double*>(partials),
+                                 static_cast<long long>(used), max_norm, out));
+    }
   }
   EO_CUDA(cudaGetLastError());
   return EO_OK;

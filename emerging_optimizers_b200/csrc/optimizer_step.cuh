@@ -751,15 +751,14 @@ __global__ void __launch_bounds__(kOptThreads)
   double acc = 0.0;
   float2 g[4];
   if (t.vec) {
+    constexpr int kDeep = 16 / sizeof(G);  // loads in flight: 128 bytes a lane
     const G* p = tg + at + 8 * lane;
-    for (; at + 3 * kOptTrip + kOptRun <= end; at += 4 * kOptTrip, p += 4 * kOptTrip) {  // four loads in flight
-      Run<G> run[4];
-      run[0].get(p);
-      run[1].template get<kOptTrip>(p);
-      run[2].template get<2 * kOptTrip>(p);
-      run[3].template get<3 * kOptTrip>(p);
+    for (; at + (kDeep - 1) * kOptTrip + kOptRun <= end; at += kDeep * kOptTrip, p += kDeep * kOptTrip) {
+      Run<G> run[kDeep];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
+      for (int i = 0; i < kDeep; ++i) run[i].get(p + i * kOptTrip);
+#pragma unroll
+      for (int i = 0; i < kDeep; ++i) {
         run[i].unpack(g);
         acc += sum_of_squares(g);
       }
@@ -781,30 +780,49 @@ __global__ void __launch_bounds__(kOptThreads)
   if (threadIdx.x == 0) partial[blockIdx.x] = total;
 }
 
-// out[0] = norm, out[1] = min(1, max_norm / (norm + 1e-6)); NaN stays NaN.
-__global__ void __launch_bounds__(kEwThreads)
+// out[0] = norm, out[1] = min(1, max_norm / (norm + 1e-6)); NaN stays NaN.  Launched ahead of the end of the kernels before it
+// and waits for them here, so that its launch costs nothing.
+constexpr int kNormThreads = 1024;
+__global__ void __launch_bounds__(kNormThreads)
     grad_norm_final_kernel(const double* __restrict__ partial, long long n, float max_norm, float* __restrict__ out) {
+  __shared__ double warp_sums[kNormThreads / 32];
+  cudaGridDependencySynchronize();
   double acc = 0.0;
-  for (long long i = threadIdx.x; i < n; i += kEwThreads) acc += partial[i];
-  const double total = block_reduce_sum(acc);
-  if (threadIdx.x == 0) {
-    const float norm = static_cast<float>(sqrt(total));
-    const float coef = __fdiv_rn(max_norm, __fadd_rn(norm, 1e-6f));
-    out[0] = norm;
-    out[1] = coef > 1.0f ? 1.0f : coef;
+  for (long long i = threadIdx.x; i < n; i += 4 * kNormThreads) {
+    double x[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) x[k] = i + k * kNormThreads < n ? __ldcg(partial + i + k * kNormThreads) : 0.0;
+    acc += (x[0] + x[1]) + (x[2] + x[3]);
+  }
+#pragma unroll
+  for (int off = 16; off > 0; off >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, off);
+  if ((threadIdx.x & 31) == 0) warp_sums[threadIdx.x >> 5] = acc;
+  __syncthreads();
+  if (threadIdx.x < 32) {
+    double total = warp_sums[threadIdx.x];
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) total += __shfl_xor_sync(0xffffffffu, total, off);
+    if (threadIdx.x == 0) {
+      const float norm = static_cast<float>(sqrt(total));
+      const float coef = __fdiv_rn(max_norm, __fadd_rn(norm, 1e-6f));
+      out[0] = norm;
+      out[1] = coef > 1.0f ? 1.0f : coef;
+    }
   }
 }
 
-// g <- g * coef; nothing to do when coef is 1.
+// g <- g * coef; nothing to do when coef is 1.  Chunks are taken from the last to the first: the end of the gradients is still in
+// L2 from the sum of squares.
 template <typename G, int kCapacity>
 __global__ void __launch_bounds__(kOptThreads)
     grad_scale_kernel(const __grid_constant__ TensorTable<GradEntry, kCapacity> table, const float* __restrict__ coef_ptr) {
   const float coef = *coef_ptr;
   if (coef == 1.0f) return;
-  const int which = find_tensor(table, blockIdx.x);
+  const uint32_t chunk = gridDim.x - 1 - blockIdx.x;
+  const int which = find_tensor(table, chunk);
   const GradEntry& t = table.t[which];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const long long begin = static_cast<long long>(blockIdx.x - table.first[which]) * table.trips * kOptTrip;
+  const long long begin = static_cast<long long>(chunk - table.first[which]) * table.trips * kOptTrip;
   const long long end = min(begin + static_cast<long long>(table.trips) * kOptTrip, t.numel);
   long long at = begin + warp * kOptRun;
   G* const tg = static_cast<G*>(t.g);

@@ -7,6 +7,7 @@ one launch for each mix of types (up to 384 tensors), whatever their sizes.
 
 from __future__ import annotations
 
+from itertools import compress
 from typing import Any, Callable, Sequence
 
 import torch
@@ -261,26 +262,25 @@ class AdamW(optim.Optimizer):
         first_index = 0
         for group in self.param_groups:
             params = [p for p in group["params"] if p.grad is not None]
-            if any(p.grad.is_sparse for p in params):
+            grads = [p.grad for p in params]
+            if any(g.is_sparse for g in grads):
                 raise RuntimeError("AdamW does not support sparse gradients")
-            for p in params:
-                if not self.state[p]:
+            states = [self.state[p] for p in params]
+            for p, state in zip(params, states):
+                if not state:
                     if p.is_cuda and torch.cuda.is_current_stream_capturing():
                         raise RuntimeError("run a step before capturing one: the state must exist when the capture begins")
-                    self.state[p] = self._new_state(p)
-            # one call per device, kind of parameter and step number (with device counters: whatever the number)
-            keys = [
-                (p.get_device(), p.dtype, 0 if self.capturable else self.state[p]["step"] + 1) for p in params
-            ]  # fmt: skip
-            for key in dict.fromkeys(keys):
-                chosen = params if keys.count(key) == len(keys) else [p for p, k in zip(params, keys) if k == key]
-                self._call(group, chosen, key[2], grad_scale, first_index)
-                first_index += len(chosen)
+                    state.update(self._new_state(p))
+            # one call per device, type of parameter and step number (with device counters: whatever the number)
+            steps = [0] * len(params) if self.capturable else [state["step"] + 1 for state in states]
+            calls = list(zip(map(torch.Tensor.get_device, params), [p.dtype for p in params], steps))
+            for call in dict.fromkeys(calls):
+                chosen = [c == call for c in calls]
+                lists = (params, grads, states) if all(chosen) else ([*compress(t, chosen)] for t in (params, grads, states))
+                first_index += self._call(group, *lists, call[2], grad_scale, first_index)
         return None
 
-    def _call(self, group, params, step, grad_scale, first_index) -> None:  # type: ignore[no-untyped-def]
-        states = [self.state[p] for p in params]
-        grads = [p.grad for p in params]
+    def _call(self, group, params, grads, states, step, grad_scale, first_index) -> int:  # type: ignore[no-untyped-def]
         plain = all(map(torch.Tensor.is_contiguous, params))
         orders = [None] * len(params) if plain else [_memory_order(p) for p in params]
         if not plain or not all(map(torch.Tensor.is_contiguous, grads)):
@@ -305,6 +305,7 @@ class AdamW(optim.Optimizer):
         if not self.capturable:
             for s in states:
                 s["step"] = step
+        return len(params)
 
     # -- checkpoints -------------------------------------------------------------------------------------------------
 
