@@ -826,18 +826,17 @@ def adamw_step(
     _check(_launch(device, lib().eo_adamw_step, n, table, config), "eo_adamw_step")
 
 
-def grad_norm(
-    index: int, device: torch.device, n: int, table: bytes, types: int, max_norm: float, in_place: bool
-) -> torch.Tensor:
-    """Norm and clipping coefficient (fp32, shape (2,)) of the ``n`` tensors of ``table`` (see ``eo_grad_norm``);
+def grad_norm(grads, device: int, table: bytes, types: int, max_norm: float, in_place: bool) -> torch.Tensor:
+    """Norm and clipping coefficient (fp32, shape (2,)) of ``grads``, whose ``table`` is (see ``eo_grad_norm``);
     ``types`` is the set of types in it, as bits; ``in_place`` also multiplies them by the coefficient."""
     global launch_count
-    out = torch.empty(2, dtype=torch.float32, device=device)
+    n = len(grads)
+    out = grads[0].new_empty(2, dtype=torch.float32)
     nbytes = lib().eo_grad_norm_scratch_bytes(n)
-    scratch = torch.empty(nbytes, dtype=torch.uint8, device=device)
+    scratch = grads[0].new_empty(nbytes, dtype=torch.uint8)
     launch_count += 1 + types.bit_count() * -(-n // MAX_TENSORS_PER_LAUNCH) * (2 if in_place else 1)
     rc = _launch(
-        index, lib().eo_grad_norm, n, table, max_norm, 1 if in_place else 0, out.data_ptr(), scratch.data_ptr(), nbytes
+        device, lib().eo_grad_norm, n, table, max_norm, 1 if in_place else 0, out.data_ptr(), scratch.data_ptr(), nbytes
     )
     _check(rc, "eo_grad_norm")
     return out

@@ -974,8 +974,9 @@ int eo_adamw_step(int n, const int64_t* host_table, const eo_adamw_config* confi
   eo::AdamWFactors* factors = device_factors ? static_cast<eo::AdamWFactors*>(cfg.scratch) : nullptr;
   for (int k = 0; k < 8; ++k) {
     if (!(kinds & (1u << k))) continue;
-    const uintptr_t ap = (k & EO_KIND_PARAM_BF16) ? 16 : 32, ag = (k & EO_KIND_GRAD_BF16) ? 16 : 32,
-                    as = cfg.state_bits == 8 ? 8 : 32;
+    const bool bits8 = cfg.state_bits == 8;  // reads through shared memory in pieces of 16 bytes
+    const uintptr_t ap = (k & EO_KIND_PARAM_BF16) || bits8 ? 16 : 32, ag = (k & EO_KIND_GRAD_BF16) || bits8 ? 16 : 32,
+                    as = bits8 ? 8 : 32;
     auto fill = [&](int i, eo::AdamWEntry& t) {
       if (numel[i] == 0 || kind[i] != k) return false;
       t.p = reinterpret_cast<void*>(p[i]);

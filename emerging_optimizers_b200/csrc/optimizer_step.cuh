@@ -62,6 +62,11 @@ struct __align__(16) Run<float> {
                  "f"(x[4]), "f"(x[5]), "f"(x[6]), "f"(x[7])
                  : "memory");
   }
+  // as put, for addresses aligned to 16 bytes only
+  __device__ __forceinline__ void put_halves(float* p) const {
+    reinterpret_cast<float4*>(p)[0] = make_float4(x[0], x[1], x[2], x[3]);
+    reinterpret_cast<float4*>(p)[1] = make_float4(x[4], x[5], x[6], x[7]);
+  }
   __device__ __forceinline__ void get_some(const float* p, long long left, int lane) {
 #pragma unroll
     for (int k = 0; k < 8; ++k) x[k] = (32 * k + lane < left) ? p[32 * k + lane] : 0.0f;
@@ -607,7 +612,10 @@ struct AdamWRing {
   }
   // The run worked on lies kAhead elements before the one to be fetched.
   __device__ __forceinline__ void put(const AdamWRun<P, G, kRemainder, true>& d, int lane) const {
-    d.p.put(reinterpret_cast<P*>(const_cast<char*>(p) + (sizeof(P) == 4 ? 16 * lane : 0)) - kAhead);
+    if constexpr (sizeof(P) == 4)
+      d.p.put_halves(reinterpret_cast<P*>(const_cast<char*>(p) + 16 * lane) - kAhead);
+    else
+      d.p.put(reinterpret_cast<P*>(const_cast<char*>(p)) - kAhead);
     if constexpr (kRemainder) d.r.put(r - kAhead);
     d.m.put(m - kAhead);
     d.v.put(v - kAhead);

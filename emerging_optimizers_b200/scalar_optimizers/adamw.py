@@ -83,7 +83,6 @@ def _step(
     )  # fmt: skip
 
 
-@torch.no_grad()
 def adamw_step(
     params: Sequence[torch.Tensor],
     grads: Sequence[torch.Tensor],
@@ -102,7 +101,7 @@ def adamw_step(
     """One AdamW step of a list of tensors, in place.
 
     All arithmetic is fp32 with one rounding per operation, the moments are fp32.  Tensors are contiguous CUDA tensors
-    of one device; parameters and gradients fp32 or bf16 in any mix.
+    of one device; parameters and gradients fp32 or bf16 in any mix.  No two tensors that are written may overlap.
 
     Args:
         params, grads, exp_avgs, exp_avg_sqs: parameters, gradients, first and second moments, one of each per tensor.
@@ -121,7 +120,6 @@ def adamw_step(
     )  # fmt: skip
 
 
-@torch.no_grad()
 def adamw_step_8bit(
     params: Sequence[torch.Tensor],
     grads: Sequence[torch.Tensor],
@@ -237,7 +235,9 @@ class AdamW(optim.Optimizer):
 
     def moments(self, p: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
         """First and second moment of ``p`` as new fp32 tensors, whatever they are stored in."""
-        state = self.state[p]
+        state = self.state.get(p)
+        if not state:
+            raise ValueError("the parameter has no state yet")
         return tuple(self._values(state, name, signed) for name, signed in (("exp_avg", True), ("exp_avg_sq", False)))  # type: ignore[return-value]
 
     @staticmethod
@@ -315,6 +315,10 @@ class AdamW(optim.Optimizer):
         Moments of the other width are converted (32 to 8 bits: rounded to nearest); types are kept as this optimizer
         has them, whatever the parameter's.
         """
+        for group in state_dict["param_groups"]:
+            for key in ("amsgrad", "maximize"):
+                if group.get(key):
+                    raise ValueError(f"the saved optimizer ran with {key}, which AdamW does not have")
         saved = state_dict["state"]
         super().load_state_dict({**state_dict, "state": {}})
         ids = [i for group in state_dict["param_groups"] for i in group["params"]]

@@ -23,7 +23,6 @@ def exponent_count(numel: int) -> int:
     return -(-numel // _native.QUANT_BLOCK)
 
 
-@torch.no_grad()
 def quantize_blockwise(
     x: torch.Tensor, *, signed: bool, seed: int | None = None
 ) -> tuple[torch.Tensor, torch.Tensor]:
@@ -40,13 +39,12 @@ def quantize_blockwise(
         raise ValueError(f"x is not contiguous (shape {tuple(x.shape)}, strides {x.stride()})")
     if seed is not None and not 0 <= seed < 1 << 32:
         raise ValueError(f"seed must be in [0, 2^32), got {seed}")
-    codes = torch.empty(x.shape, dtype=torch.uint8, device=x.device)
-    exponents = torch.empty(exponent_count(x.numel()), dtype=torch.uint8, device=x.device)
+    codes = torch.empty_like(x, dtype=torch.uint8)
+    exponents = x.new_empty(exponent_count(x.numel()), dtype=torch.uint8)
     _native.quantize_blockwise(x, signed, seed, codes, exponents)
     return codes, exponents
 
 
-@torch.no_grad()
 def dequantize_blockwise(
     codes: torch.Tensor, exponents: torch.Tensor, *, signed: bool, dtype: torch.dtype = torch.float32
 ) -> torch.Tensor:
@@ -61,6 +59,6 @@ def dequantize_blockwise(
         raise ValueError(f"exponents must be {exponent_count(codes.numel())} bytes on {codes.device}")
     if not (codes.is_contiguous() and exponents.is_contiguous()):
         raise ValueError("codes and exponents must be contiguous")
-    out = torch.empty(codes.shape, dtype=dtype, device=codes.device)
+    out = torch.empty_like(codes, dtype=dtype)
     _native.dequantize_blockwise(codes, exponents, signed, out)
     return out

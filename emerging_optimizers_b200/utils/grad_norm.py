@@ -23,17 +23,15 @@ def _norm(grads: Sequence[torch.Tensor], max_norm: float, in_place: bool) -> tor
         raise ValueError(f"max_norm must not be negative, got {max_norm}")
     grads = list(grads)
     device, table, types = _native.host().grads_table(grads, in_place)
-    return _native.grad_norm(device, grads[0].device, len(grads), table, types, max_norm, in_place)
+    return _native.grad_norm(grads, device, table, types, max_norm, in_place)
 
 
-@torch.no_grad()
 def global_grad_norm(grads: Sequence[torch.Tensor]) -> torch.Tensor:
     """2-norm of all elements of ``grads`` (contiguous fp32 or bf16 CUDA tensors of one device) as an fp32 scalar
     tensor.  Squares are summed in float64 in a fixed order: the same call gives the same bits."""
     return _norm(grads, math.inf, False)[0]
 
 
-@torch.no_grad()
 def clip_coefficient(grads: Sequence[torch.Tensor], max_norm: float) -> tuple[torch.Tensor, torch.Tensor]:
     """``(norm, min(1, max_norm / (norm + 1e-6)))`` as fp32 scalar tensors on the device; the gradients stay as they are.
 
@@ -43,7 +41,6 @@ def clip_coefficient(grads: Sequence[torch.Tensor], max_norm: float) -> tuple[to
     return norm, coefficient
 
 
-@torch.no_grad()
 def clip_grads_(grads: Sequence[torch.Tensor], max_norm: float) -> torch.Tensor:
     """Multiply all of ``grads`` in place by ``min(1, max_norm / (norm + 1e-6))``; returns the norm from before."""
     return _norm(grads, max_norm, True)[0]

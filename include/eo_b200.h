@@ -404,7 +404,8 @@ enum { EO_KIND_PARAM_BF16 = 1, EO_KIND_GRAD_BF16 = 2, EO_KIND_REMAINDER = 4 };
  * exponent bytes of the first and of the second moments (8-bit states, else 0), remainders (or 0), device step counters
  * (int64, or 0), then the element counts and the kinds (EO_KIND_* flags; 0: fp32 parameters and gradients).  Tensors are
  * flat and dense, any alignment of their element type; the wide accesses are used where p, g, m, v and remainders are
- * aligned for eight elements (fp32: 32 bytes, 16-bit types: 16, codes: 8).  Empty tensors are skipped.
+ * aligned for eight elements (fp32: 32 bytes, 16 with 8-bit states; 16-bit types: 16, codes: 8).  Empty tensors are skipped;
+ * no two tensors that are written may overlap.
  *
  * state_bits 32: m, v fp32.  state_bits 8: m, v are codes of one byte per element with one exponent byte per 256
  * elements (see eo_quantize_blockwise), rounded at random with bits from (seed, first_index + place in the list, step,

@@ -245,22 +245,24 @@ def test_adamw_8bit_is_the_32bit_step_between_decoding_and_rounding(p_dtype, g_d
             assert np.array_equal(codes.cpu().numpy(), want)
 
 
-@pytest.mark.parametrize("off", [1, 4, 8])
-def test_adamw_8bit_at_any_alignment_gives_the_same_bits(off):
-    n = 3001
-    (p,), (g,), (m,), (v,) = _inputs([n])
+@pytest.mark.parametrize("n", [3001, 70_000])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("off,off_codes", [(1, 1), (4, 4), (4, 0), (8, 8), (0, 1)])
+def test_adamw_8bit_at_any_alignment_gives_the_same_bits(off, off_codes, dtype, n):
+    (p,), (g,), (m,), (v,) = _inputs([n], dtype, dtype)
     (mc,), (me,) = _quantized([m], True)
     (vc,), (ve,) = _quantized([v], False)
     moved = []
     for t in (p, g, mc, me, vc, ve):
+        o = off_codes if t.dtype == torch.uint8 else off
         room = torch.full((t.numel() + 16,), 9, dtype=t.dtype, device="cuda")
-        room[off : off + t.numel()] = t
-        moved.append((room, room[off : off + t.numel()]))
+        room[o : o + t.numel()] = t
+        moved.append((room, room[o : o + t.numel()], o))
     adamw_step_8bit([p], [g], [mc], [me], [vc], [ve], **HYPER, step=3, seed=2)
-    adamw_step_8bit(*[[view] for _, view in moved], **HYPER, step=3, seed=2)
-    for t, (room, view) in zip((p, g, mc, me, vc, ve), moved):
+    adamw_step_8bit(*[[view] for _, view, _ in moved], **HYPER, step=3, seed=2)
+    for t, (room, view, o) in zip((p, g, mc, me, vc, ve), moved):
         assert _same(t, view)
-        assert bool((room[:off] == 9).all()) and bool((room[off + t.numel() :] == 9).all())
+        assert bool((room[:o] == 9).all()) and bool((room[o + t.numel() :] == 9).all())
 
 
 def test_random_bits_depend_on_seed_step_and_place():
@@ -635,6 +637,81 @@ def test_other_streams():
     torch.cuda.current_stream().wait_stream(side)
     assert all(_same(a[0], b[0]) for a, b in zip(lists, other))
     assert _same(norm, utils.global_grad_norm(lists[1]))
+
+
+def test_two_captured_graphs_replayed_at_once():
+    """Two graphs of different parameters share no workspace: replayed on two streams they give what they give alone."""
+    def build():
+        lists = _inputs([300_000, 77])
+        grads = lists[1]
+        step = torch.ones((), dtype=torch.int64, device="cuda")
+        def body():
+            norm, coef = utils.clip_coefficient(grads, 1e-2)
+            adamw_step(*lists, **HYPER, step=step, grad_scale=coef)
+            return norm
+        return lists, body
+
+    want, body = build()
+    norm = body()
+    torch.cuda.synchronize()
+    sides = []
+    for _ in range(2):
+        lists, body = build()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = body()
+        sides.append((lists, graph, out, torch.cuda.Stream()))
+    torch.cuda.synchronize()
+    for _, graph, _, stream in sides:
+        with torch.cuda.stream(stream):
+            graph.replay()
+    torch.cuda.synchronize()
+    for lists, _, out, _ in sides:
+        assert _same(out, norm)
+        assert all(_same(x, y) for k in (0, 2, 3) for x, y in zip(lists[k], want[k]))
+
+
+def test_many_calls_queued_without_waiting():
+    """Workspaces of one call are handed to the next by the allocator while the first still runs."""
+    gs = [[_randn(1 << 20, i, 0.1 * (i + 1))] for i in range(8)]
+    want = [_norm64(g) for g in gs]
+    norms = [utils.global_grad_norm(gs[i % 8]) for i in range(200)]
+    for i, n in enumerate(norms):
+        assert abs(float(n) - want[i % 8]) <= 2 * ULP * want[i % 8]
+
+
+def test_zero_dimensional_and_empty_parameters():
+    params = [torch.nn.Parameter(t) for t in (torch.tensor(2.0, device="cuda"), torch.empty(0, 3, device="cuda"), torch.ones(1, 1, device="cuda"))]
+    for bits in (32, 8):
+        opt = AdamW(params, lr=0.1, weight_decay=0.0, state_bits=bits)
+        for p in params:
+            p.grad = torch.ones_like(p)
+        before = [p.detach().clone() for p in params]
+        opt.step()
+        for p, b in zip(params, before):  # the first step moves by lr, whatever the gradient's size
+            assert torch.allclose(p.detach(), b - 0.1, rtol=0, atol=1e-6)
+        opt.load_state_dict(opt.state_dict())
+        assert utils.clip_grad_norm_(params, 1e-3) is not None
+
+
+def test_unknown_states_are_refused():
+    p = torch.nn.Parameter(torch.ones(4, device="cuda"))
+    p.grad = torch.ones_like(p)
+    opt = AdamW([p])
+    with pytest.raises(ValueError, match="no state"):
+        opt.moments(p)
+    assert p not in opt.state
+    for key in ("amsgrad", "maximize"):
+        other = torch.optim.AdamW([p], **{key: True})
+        other.step()
+        with pytest.raises(ValueError, match=key):
+            opt.load_state_dict(other.state_dict())
+    wrong = torch.nn.Parameter(torch.ones(5, device="cuda"))
+    wrong.grad = torch.ones_like(wrong)
+    third = AdamW([wrong])
+    third.step()
+    with pytest.raises(ValueError, match="does not fit"):
+        opt.load_state_dict(third.state_dict())
 
 
 def test_autograd_sees_the_step():
