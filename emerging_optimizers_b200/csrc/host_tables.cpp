@@ -21,22 +21,29 @@ constexpr int64_t kBlock = 256;  // elements that share an exponent byte of an 8
 // A Python error is set.
 struct Raised {};
 
+class Owned {  // a new reference; a null one means that a Python error is set
+ public:
+  explicit Owned(PyObject* object) : object_(object) {
+    if (object_ == nullptr) throw Raised{};
+  }
+  ~Owned() { Py_DECREF(object_); }
+  Owned(const Owned&) = delete;
+  PyObject* get() const { return object_; }
+
+ private:
+  PyObject* object_;
+};
+
 [[noreturn]] void raise(PyObject* type, const std::string& text) {
   PyErr_SetString(type, text.c_str());
   throw Raised{};
 }
 
 [[noreturn]] void raise_no_cpu_path(const std::string& name, const at::Tensor& t) {
-  PyObject* module = PyImport_ImportModule("emerging_optimizers_b200._native");
-  PyObject* type = module != nullptr ? PyObject_GetAttrString(module, "NativeLibraryError") : nullptr;
-  Py_XDECREF(module);
-  if (type != nullptr) {
-    PyErr_SetString(type, (name + " is on " + t.device().str() +
-                           "; emerging_optimizers_b200 runs on CUDA sm_100 devices only (there is no CPU path).")
-                              .c_str());
-    Py_DECREF(type);
-  }
-  throw Raised{};
+  Owned module(PyImport_ImportModule("emerging_optimizers_b200._native"));
+  Owned type(PyObject_GetAttrString(module.get(), "NativeLibraryError"));
+  raise(type.get(), name + " is on " + t.device().str() +
+                        "; emerging_optimizers_b200 runs on CUDA sm_100 devices only (there is no CPU path).");
 }
 
 enum Types : unsigned { kF32 = 1, kBF16 = 2, kU8 = 4, kI16 = 8, kI64 = 16 };
@@ -71,6 +78,7 @@ class Tensors {
   ~Tensors() { Py_XDECREF(seq_); }
   Tensors(const Tensors&) = delete;
   int64_t size() const { return PySequence_Fast_GET_SIZE(seq_); }
+  PyObject* item(int64_t i) const { return PySequence_Fast_GET_ITEM(seq_, i); }
   const at::Tensor& operator[](int64_t i) const {
     PyObject* item = PySequence_Fast_GET_ITEM(seq_, i);
     if (!THPVariable_Check(item)) raise(PyExc_TypeError, at(i) + " is not a tensor");
@@ -185,10 +193,8 @@ PyObject* adamw_table(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     }
     if (with_steps) {
       if (THPVariable_Check(args[7])) {
-        PyObject* one = PyTuple_Pack(1, args[7]);
-        if (one == nullptr) throw Raised{};
-        Tensors s(one, "step");
-        Py_DECREF(one);  // s holds it
+        Owned one(PyTuple_Pack(1, args[7]));
+        Tensors s(one.get(), "step");
         std::fill_n(column(7), n, address(s, 0, device, kI64, 1));
       } else {
         Tensors s(args[7], "step");
@@ -198,7 +204,8 @@ PyObject* adamw_table(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     }
     require_distinct(written, "the parameters and their state");
     for (int64_t i = 0; i < n; ++i) mark_written(p[i]);
-    return Py_BuildValue("iNI", device, bytes_of(table), kinds);
+    Owned bytes(bytes_of(table));
+    return Py_BuildValue("iOI", device, bytes.get(), kinds);
   });
 }
 
@@ -207,7 +214,7 @@ PyObject* grads_table(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   return guarded([&]() -> PyObject* {
     if (nargs != 2) raise(PyExc_TypeError, "grads_table takes 2 arguments");
     Tensors g(args[0], "grads");
-    const bool in_place = PyObject_IsTrue(args[1]) == 1;
+    const bool in_place = args[1] == Py_True;
     const int64_t n = g.size();
     if (n == 0) raise(PyExc_ValueError, "no gradients given");
     const int device = first_device(g);
@@ -223,7 +230,30 @@ PyObject* grads_table(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     require_distinct(written, "the gradients");
     if (in_place)
       for (int64_t i = 0; i < n; ++i) mark_written(g[i]);
-    return Py_BuildValue("iNI", device, bytes_of(table), types);
+    Owned bytes(bytes_of(table));
+    return Py_BuildValue("iOI", device, bytes.get(), types);
+  });
+}
+
+// with_grads(params) -> (those with a gradient, their gradients, whether all of both are contiguous and the parameters of one device
+// and type).
+PyObject* with_grads(PyObject*, PyObject* arg) {
+  return guarded([&]() -> PyObject* {
+    Tensors p(arg, "params");
+    Owned params(PyList_New(0)), grads(PyList_New(0));
+    bool uniform = true;
+    const at::Tensor* first = nullptr;
+    for (int64_t i = 0; i < p.size(); ++i) {
+      const at::Tensor& t = p[i];
+      const at::Tensor& g = t.grad();
+      if (!g.defined()) continue;
+      if (g.layout() != at::kStrided) raise(PyExc_RuntimeError, "AdamW does not support sparse gradients");
+      if (first == nullptr) first = &t;
+      uniform = uniform && t.is_contiguous() && g.is_contiguous() && t.device() == first->device() && t.scalar_type() == first->scalar_type();
+      Owned wrapped(THPVariable_Wrap(g));
+      if (PyList_Append(params.get(), p.item(i)) != 0 || PyList_Append(grads.get(), wrapped.get()) != 0) throw Raised{};
+    }
+    return Py_BuildValue("OOO", params.get(), grads.get(), uniform ? Py_True : Py_False);
   });
 }
 
@@ -245,6 +275,7 @@ PyObject* stream(PyObject*, PyObject* arg) {
 PyMethodDef methods[] = {
     {"adamw_table", reinterpret_cast<PyCFunction>(adamw_table), METH_FASTCALL, nullptr},
     {"grads_table", reinterpret_cast<PyCFunction>(grads_table), METH_FASTCALL, nullptr},
+    {"with_grads", with_grads, METH_O, nullptr},
     {"stream", stream, METH_O, nullptr},
     {nullptr, nullptr, 0, nullptr},
 };

@@ -261,29 +261,29 @@ class AdamW(optim.Optimizer):
             raise ValueError("closure is not supported")
         first_index = 0
         for group in self.param_groups:
-            params = [p for p in group["params"] if p.grad is not None]
-            grads = [p.grad for p in params]
-            if any(g.is_sparse for g in grads):
-                raise RuntimeError("AdamW does not support sparse gradients")
+            params, grads, uniform = _native.host().with_grads(group["params"])
             states = [self.state[p] for p in params]
-            for p, state in zip(params, states):
-                if not state:
-                    if p.is_cuda and torch.cuda.is_current_stream_capturing():
-                        raise RuntimeError("run a step before capturing one: the state must exist when the capture begins")
-                    state.update(self._new_state(p))
+            if not all(states):
+                for p, state in zip(params, states):
+                    if not state:
+                        if p.is_cuda and torch.cuda.is_current_stream_capturing():
+                            raise RuntimeError("run a step before capturing one: the state must exist when the capture begins")
+                        state.update(self._new_state(p))
             # one call per device, type of parameter and step number (with device counters: whatever the number)
             steps = [0] * len(params) if self.capturable else [state["step"] + 1 for state in states]
+            if uniform and len(set(steps)) == 1:
+                first_index += self._call(group, params, grads, states, True, steps[0], grad_scale, first_index)
+                continue
             calls = list(zip(map(torch.Tensor.get_device, params), [p.dtype for p in params], steps))
             for call in dict.fromkeys(calls):
                 chosen = [c == call for c in calls]
-                lists = (params, grads, states) if all(chosen) else ([*compress(t, chosen)] for t in (params, grads, states))
-                first_index += self._call(group, *lists, call[2], grad_scale, first_index)
+                lists = ([*compress(t, chosen)] for t in (params, grads, states))
+                first_index += self._call(group, *lists, uniform, call[2], grad_scale, first_index)
         return None
 
-    def _call(self, group, params, grads, states, step, grad_scale, first_index) -> int:  # type: ignore[no-untyped-def]
-        plain = all(map(torch.Tensor.is_contiguous, params))
-        orders = [None] * len(params) if plain else [_memory_order(p) for p in params]
-        if not plain or not all(map(torch.Tensor.is_contiguous, grads)):
+    def _call(self, group, params, grads, states, plain, step, grad_scale, first_index) -> int:  # type: ignore[no-untyped-def]
+        if not plain:
+            orders = [_memory_order(p) for p in params]
             grads = [_flat(g, o) for g, o in zip(grads, orders)]
 
         def column(name):  # type: ignore[no-untyped-def]
