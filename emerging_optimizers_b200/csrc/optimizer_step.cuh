@@ -23,7 +23,9 @@ namespace eo {
 constexpr int kOptThreads = 256;
 constexpr int kOptRun = 256;                                  // elements a warp takes at a time; block of an 8-bit state
 constexpr int kOptTrip = kOptThreads / 32 * kOptRun;          // elements a CTA takes per trip
-constexpr int kOptSmallTable = 24, kOptLargeTable = 384;      // tensors per launch
+// Tensors per launch: the large table fills the 32 KB that a launch may carry, and carrying it costs the host 4 us more
+// than the 2 KB of the small one (24 tensors 8.8 us a call, 25 tensors 12.7 us).
+constexpr int kOptSmallTable = 24, kOptLargeTable = 384;
 
 // ---- memory access ---------------------------------------------------------------------------------------------------
 // A lane's eight elements of a run as they lie in memory.  get / put: elements 8 l .. 8 l + 7 from their own address (plus
@@ -559,10 +561,12 @@ struct AdamWCursor {
   }
 };
 
-// Runs of the 8-bit step on their way through shared memory: a warp's own ring of kRingStages runs, filled by asynchronous copies
-// several trips ahead.  The step keeps about 60 instructions an element between a load and its store, at 24 warps an SM too few
-// bytes are in flight otherwise.
-constexpr int kRingStages = 4;
+// Runs of the 8-bit step on their way through shared memory: a warp's own ring of kRingStages runs, filled by asynchronous
+// copies two trips ahead.  Without it the loads wait for the 60 instructions an element that lie between a load and its
+// store, and prefetching into registers costs the occupancy it should replace: 268 M fp32 elements 1028 us without, 650 us
+// with the ring.  Three stages leave room for three CTAs an SM with fp32 types; four (two CTAs) are 4 % slower under a
+// sustained load, two 3 % slower with bf16 gradients.
+constexpr int kRingStages = 3;
 template <typename P, typename G, bool kRemainder>
 struct AdamWRing {
   static constexpr int kP = 0, kG = kP + kOptRun * sizeof(P), kM = kG + kOptRun * sizeof(G), kV = kM + kOptRun,
@@ -623,10 +627,13 @@ struct AdamWRing {
 };
 
 // kRemainder: p is bf16 with remainders.  k8: m and v are codes with exponent bytes.
-// Bound by HBM with fp32 moments (28 bytes an element: 99 % of the copy bandwidth on 268 M elements, bf16 types 95 %).  With
-// 8-bit moments an element costs about 55 instructions for its 10 to 16 bytes: 97 % (fp32 types), 94 % (bf16 gradients), 89 %
-// (bf16 with remainders) and 71 % (bf16), the last bound by the issue slots.  Three CTAs an SM (80 registers): two are 6 - 12 %
-// slower with bf16 types, four spill.
+// fp32 moments: bound by HBM.  268 M elements: fp32 types 1.13 ms (28 bytes an element, 6.65 TB/s), bf16 gradients 1.06 ms
+// (6.6), bf16 0.92 ms (6.4), bf16 with remainders 1.09 ms (6.4).
+// 8-bit moments: 60 instructions an element for its 10 to 16 bytes.  fp32 types 0.65 ms (6.6 TB/s), bf16 gradients 0.59 ms (6.3),
+// bf16 with remainders 0.65 ms (5.8) and bf16 0.63 ms (4.3): the last is bound by the issue slots (78 % used, the integer
+// multiply pipe 73 %).  These are bursts; run without a pause the 8-bit step reaches the GPU's power limit and its clock falls
+// from 1.97 to 1.6 GHz (fp32 types 0.74 ms), the others do not slow down.
+// Three CTAs an SM (80 registers): two are 6 - 12 % slower with bf16 types, four spill.
 template <typename P, typename G, bool kRemainder, bool k8, int kCapacity>
 __global__ void __launch_bounds__(kOptThreads, 3)
     adamw_kernel(const __grid_constant__ TensorTable<AdamWEntry, kCapacity> table, const __grid_constant__ AdamWScalars c) {

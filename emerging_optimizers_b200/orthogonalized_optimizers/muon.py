@@ -74,7 +74,7 @@ class Muon(OrthogonalizedOptimizer[HookStateT]):
     EMA momentum (optionally Nesterov), then every 2-D update is replaced by an approximation of its nearest
     semi-orthogonal matrix computed by Newton-Schulz iteration on tensor cores, scaled, and applied with decoupled
     weight decay.  Use it for hidden 2-D weights only; embeddings, the output layer and 1-D parameters belong to a
-    standard optimizer.
+    standard optimizer (:class:`emerging_optimizers_b200.scalar_optimizers.AdamW`).
 
     Args:
         {_args_doc}
