@@ -965,6 +965,9 @@ int eo_adamw_step(int n, const int64_t* host_table, const eo_adamw_config* confi
   c.eps = static_cast<float>(cfg.eps);
   c.l2 = cfg.decay_method == eo::kDecayL2 ? static_cast<float>(cfg.weight_decay) : 0.0f;
   c.minus_zero = -0.0f;
+  const bool small_eps = cfg.eps < 1e-10;
+  c.root_scale = small_eps ? -0x1p36f : -1.0f;
+  c.root_unscale = small_eps ? 0x1p-18f : 1.0f;
   c.seed = cfg.seed;
   c.f = eo::AdamWFactors{};
   if (!device_factors)

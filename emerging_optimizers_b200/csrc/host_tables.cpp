@@ -72,6 +72,7 @@ std::string names_of(unsigned types) {
 class Tensors {
  public:
   Tensors(PyObject* object, const char* name) : name_(name) {
+    if (THPVariable_Check(object)) raise(PyExc_TypeError, name_ + " must be a list of tensors, not a tensor");
     seq_ = PySequence_Fast(object, "expected a list of tensors");
     if (seq_ == nullptr) throw Raised{};
   }

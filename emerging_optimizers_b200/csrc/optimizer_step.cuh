@@ -405,6 +405,7 @@ struct AdamWFactors {
 
 struct AdamWScalars {
   float beta1, one_minus_beta1, beta2, one_minus_beta2, eps, l2, minus_zero;
+  float root_scale, root_unscale;  // the root is taken of -root_scale v and multiplied by root_unscale
   uint32_t seed;
   AdamWFactors f;             // used when dev_factors is nullptr
   const AdamWFactors* dev_factors;  // per tensor of this launch, from adamw_factors_kernel
@@ -459,22 +460,24 @@ __device__ __forceinline__ float at_least(float x, float low) {  // NaN stays Na
 // Root and quotient are rounded to nearest too, without the branches and the range checks of the compiler's, which run the
 // eight elements of a lane one after the other: one Newton step each on the hardware's approximations, its residual exact
 // through the fused multiply-add (Markstein, IBM J. Res. Dev. 34, 1990).  Compared with __fsqrt_rn on every positive float: the
-// same where the operand is at least 2^-102, within 3e-7 below; with __fdiv_rn on 3.4e10 pairs of mantissas: the same, and the
-// reciprocal inside is the nearest for every mantissa.  The root is taken of 2^24 v, so that it is exact for every normal
-// v; what overflows (v > 2^104) counts as the largest finite number, zero gives zero.  Negated operands (-v, -root,
-// -denominator) save the sign changes that the paired instructions do not have.
+// same where the operand is at least 2^-102; with __fdiv_rn on 3.4e10 pairs of mantissas: the same, and the reciprocal inside is
+// the nearest for every mantissa.  Below 2^-102 a root does not count beside an eps of 1e-10 and more.  Where eps is smaller the
+// root is taken of 2^36 v: right within three roundings down to the smallest subnormal v (the 2^-126 that keeps the
+// approximation of zero finite is 2^-13 of it then, and the Newton step squares that), and what lies above 2^92 counts as
+// the largest finite number, as infinity does otherwise.  Zero gives zero.  Negated operands (-v, -root, -denominator) save the
+// sign changes that the paired instructions do not have.
 __device__ __forceinline__ void adamw_update(float2 (&p)[4], const float2 (&g_in)[4], float2 (&m)[4], float2 (&v)[4],
                                              const AdamWScalars& c, const AdamWFactors& f, float grad_scale) {
   const float2 scale = both(grad_scale), b1 = both(c.beta1), ob1 = both(c.one_minus_beta1), b2 = both(c.beta2);
   const float2 ob2 = both(c.one_minus_beta2), l2 = both(c.l2), eps = both(-c.eps), decay = both(f.decay);
-  const float2 size = both(-f.step_size), inv = both(f.inv_root_bc2 * 0x1p-12f), mz = both(c.minus_zero);
+  const float2 size = both(-f.step_size), inv = both(f.inv_root_bc2 * c.root_unscale), mz = both(c.minus_zero);
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
     float2 g = product(g_in[k], scale, mz);
     if (c.l2 != 0.0f) g = add2(g, product(p[k], l2, mz));
     m[k] = add2(product(m[k], b1, mz), product(g, ob1, mz));
     v[k] = add2(product(v[k], b2, mz), product(product(g, g, mz), ob2, mz));
-    float2 nv = mul2(v[k], both(-0x1p24f));
+    float2 nv = mul2(v[k], both(c.root_scale));
     nv.x = at_least(nv.x, -3.4028234664e38f);
     nv.y = at_least(nv.y, -3.4028234664e38f);
     const float2 above_zero = add2(nv, both(-0x1p-126f));

@@ -55,9 +55,10 @@ def _step(
     _check_hyperparameters(lr, betas, eps, weight_decay, weight_decay_method)
     if not (0 <= seed <= _MASK32):
         raise ValueError(f"seed must be in [0, 2^32), got {seed}")
-    params = list(params)
-    if not params:
-        return
+    if not torch.is_tensor(params):  # a tensor would be taken apart into its rows: the table refuses it
+        params = list(params)
+        if not params:
+            return
     on_host = isinstance(step, int)
     if on_host and step < 1:
         raise ValueError(f"step counts from 1, got {step}")
@@ -296,12 +297,18 @@ class AdamW(optim.Optimizer):
         exponents = [None, None]
         if self.state_bits == 8:
             exponents = [[s[name] for s in states] for name in ("exp_avg_exponents", "exp_avg_sq_exponents")]
-        _step(
-            params if plain else [_flat(p, o) for p, o in zip(params, orders)], grads, column("exp_avg"), column("exp_avg_sq"),
-            *exponents, column("remainder") if self._has_remainder(params[0]) else None, lr=group["lr"],
-            betas=group["betas"], eps=group["eps"], weight_decay=group["weight_decay"], step=step,
-            weight_decay_method=self.weight_decay_method, grad_scale=grad_scale, seed=self.seed, first_index=first_index,
-        )  # fmt: skip
+        try:
+            _step(
+                params if plain else [_flat(p, o) for p, o in zip(params, orders)], grads, column("exp_avg"),
+                column("exp_avg_sq"), *exponents, column("remainder") if self._has_remainder(params[0]) else None,
+                lr=group["lr"], betas=group["betas"], eps=group["eps"], weight_decay=group["weight_decay"], step=step,
+                weight_decay_method=self.weight_decay_method, grad_scale=grad_scale, seed=self.seed,
+                first_index=first_index,
+            )  # fmt: skip
+        except Exception:
+            if self.capturable:  # a step that was refused does not count
+                torch._foreach_sub_(step, 1)
+            raise
         if not self.capturable:
             for s in states:
                 s["step"] = step

@@ -21,7 +21,8 @@ __all__ = ["clip_coefficient", "clip_grad_norm_", "clip_grads_", "global_grad_no
 def _norm(grads: Sequence[torch.Tensor], max_norm: float, in_place: bool) -> torch.Tensor:
     if not max_norm >= 0.0:
         raise ValueError(f"max_norm must not be negative, got {max_norm}")
-    grads = list(grads)
+    if not torch.is_tensor(grads):  # a tensor would be taken apart into its rows: the table refuses it
+        grads = list(grads)
     device, table, types = _native.host().grads_table(grads, in_place)
     return _native.grad_norm(grads, device, table, types, max_norm, in_place)
 

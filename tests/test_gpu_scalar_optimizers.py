@@ -125,6 +125,31 @@ def test_adamw_step_at_any_alignment_gives_the_same_bits(off, dtype):
         assert bool((room[:o] == 9).all()) and bool((room[o + n :] == 9).all())  # nothing beside it was written
 
 
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("size,eps", [(1e18, 1e-8), (1e12, 1e-8), (1e-15, 1e-8), (1e-15, 0.0), (1e-18, 1e-30), (3e-21, 0.0)])
+def test_gradients_of_any_size(size, eps, bits):
+    """First steps on gradients whose squares reach the ends of the fp32 range: against float64 from the moments that the
+    fp32 step leaves (their own rounding, of subnormal numbers among them, is not in question here)."""
+    n = 2000
+    g = _randn(n, 3, size)
+    p = torch.zeros(n, device="cuda")
+    m, v = torch.zeros(n, device="cuda"), torch.zeros(n, device="cuda")
+    hyper = dict(lr=1e-2, betas=(0.9, 0.95), eps=eps, weight_decay=0.0)
+    adamw_step([p], [g], [m], [v], **hyper, step=1)
+    if bits == 8:
+        q = torch.zeros(n, device="cuda")
+        state = [[torch.zeros(k, dtype=torch.uint8, device="cuda")] for k in (n, 8, n, 8)]
+        adamw_step_8bit([q], [g], *state, **hyper, step=1, seed=0)
+        assert _same(q, p)
+    m64, v64 = _np64(m), _np64(v)
+    some = (v64 > 0) & np.isfinite(v64)
+    assert some.mean() > 0.5
+    want = -(1e-2 / (1 - 0.9)) * m64[some] / (np.sqrt(v64[some] / (1 - 0.95)) + eps)
+    # the root, three products, a sum, the quotient, two factors: at most ten roundings; 3e-7 (five roundings) for a root below
+    # 2^-102, and the rounding of a parameter that may itself be subnormal
+    assert np.all(np.abs(_np64(p)[some] - want) <= 15 * ULP * np.abs(want) + 2.0**-149)
+
+
 def test_adamw_first_step_and_empty_lists():
     p, g = _randn(300, 1), _randn(300, 2)
     m, v = torch.zeros_like(p), torch.zeros_like(p)
@@ -511,6 +536,27 @@ def test_checkpoint_resumes_bit_for_bit(bits, dtype):
             assert _same(value, other) if torch.is_tensor(value) else value == other
 
 
+@pytest.mark.parametrize("source,target", [(True, False), (False, True)])
+def test_checkpoint_between_host_and_device_counters(source, target):
+    a = _model_params()
+    first = AdamW(a, lr=1e-2, capturable=source)
+    for step in range(3):
+        _set_grads(a, step)
+        first.step()
+    b = [torch.nn.Parameter(p.detach().clone()) for p in a]
+    second = AdamW(b, lr=1e-2, capturable=target)
+    second.load_state_dict(first.state_dict())
+    for params, opt in ((a, first), (b, second)):
+        _set_grads(params, 9)
+        opt.step()
+    for p, q in zip(a, b):
+        assert int(first.state[p]["step"]) == int(second.state[q]["step"]) == 4
+        for x, y in zip(first.moments(p), second.moments(q)):
+            assert _same(x, y)
+        # the factors may differ in their last place (see the test of device counters)
+        assert torch.allclose(p.detach(), q.detach(), rtol=4 * ULP, atol=4 * 3 * ULP * 1e-2)
+
+
 def test_checkpoints_move_between_widths():
     a = _model_params(BF16)
     wide = AdamW(a, lr=1e-2, master_remainder=True)
@@ -767,7 +813,23 @@ def test_refusals_on_the_gpu():
         dequantize_blockwise(u8[0], e8[0], signed=True, dtype=torch.float16)
     with pytest.raises(ValueError, match="exponents"):
         dequantize_blockwise(u8[0], u8[1], signed=True)
-    for t in [x, *y]:
+    z = torch.zeros(4, 8, device="cuda")
+    with pytest.raises(TypeError, match="list of tensors"):
+        adamw_step(z, z.clone(), z.clone(), z.clone(), **kw)
+    with pytest.raises(TypeError, match="list of tensors"):
+        adamw_step([z], z.clone(), [z.clone()], [z.clone()], **kw)
+    with pytest.raises(TypeError, match="list of tensors"):
+        utils.clip_grads_(z, 1.0)
+    with pytest.raises(TypeError, match="not a tensor"):
+        adamw_step([x], [None], [y[0]], [y[1]], **kw)
+    p = torch.nn.Parameter(torch.zeros(8, device="cuda"))
+    p.grad = torch.zeros(8, device="cuda")
+    opt = AdamW([p], capturable=True)
+    opt.step()
+    with pytest.raises(TypeError, match="grad_scale"):
+        opt.step(grad_scale=2.0)
+    assert int(opt.state[p]["step"]) == 1  # a step that was refused does not count
+    for t in [x, *y, z]:
         assert not bool(t.any())  # no call wrote anything
 
 
