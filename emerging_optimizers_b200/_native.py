@@ -114,7 +114,7 @@ _PROTOTYPES: dict[str, tuple] = {
     ),
     "eo_adamw_scratch_bytes": (c_size_t, [c_int]),
     "eo_adamw_step": (c_int, [c_int, c_char_p, c_char_p, c_void_p]),
-    "eo_grad_norm_scratch_bytes": (c_size_t, [c_int]),
+    "eo_grad_norm_scratch_bytes": (c_size_t, [c_int, c_int64]),
     "eo_grad_norm": (c_int, [c_int, c_char_p, c_float, c_int, c_void_p, c_void_p, c_size_t, c_void_p]),
     "eo_quantize_blockwise": (
         c_int,
@@ -826,18 +826,25 @@ def adamw_step(
     _check(_launch(device, lib().eo_adamw_step, n, table, config), "eo_adamw_step")
 
 
-def grad_norm(grads, device: int, table: bytes, types: int, max_norm: float, in_place: bool) -> torch.Tensor:
-    """Norm and clipping coefficient (fp32, shape (2,)) of ``grads``, whose ``table`` is (see ``eo_grad_norm``);
-    ``types`` is the set of types in it, as bits; ``in_place`` also multiplies them by the coefficient."""
+def grad_norm(
+    grads, device: int, table: bytes, types: int, elements: int, max_norm: float, in_place: bool
+) -> torch.Tensor:
+    """Norm and clipping coefficient of ``grads``, whose ``table`` is (see ``eo_grad_norm``) and whose elements add up to
+    ``elements``, as the first two elements of an fp32 tensor; ``types`` is the set of types in it, as bits; ``in_place`` also
+    multiplies them by the coefficient."""
     global launch_count
     n = len(grads)
-    out = grads[0].new_empty(2, dtype=torch.float32)
-    nbytes = lib().eo_grad_norm_scratch_bytes(n)
-    scratch = grads[0].new_empty(nbytes, dtype=torch.uint8)
+    nbytes = lib().eo_grad_norm_scratch_bytes(n, elements)
+    # the partial sums of a small set lie behind the result: one allocation less, and little for the result to keep alive
+    apart = nbytes > 8192
+    out = grads[0].new_empty(2 if apart else 2 + nbytes // 4, dtype=torch.float32)
+    scratch = grads[0].new_empty(nbytes, dtype=torch.uint8) if apart else None
     launch_count += 1 + types.bit_count() * -(-n // MAX_TENSORS_PER_LAUNCH) * (2 if in_place else 1)
+    ptr = out.data_ptr()
     rc = _launch(
-        device, lib().eo_grad_norm, n, table, max_norm, 1 if in_place else 0, out.data_ptr(), scratch.data_ptr(), nbytes
-    )
+        device, lib().eo_grad_norm, n, table, max_norm, 1 if in_place else 0, ptr,
+        ptr + 8 if scratch is None else scratch.data_ptr(), nbytes,
+    )  # fmt: skip
     _check(rc, "eo_grad_norm")
     return out
 

@@ -1005,10 +1005,11 @@ int eo_adamw_step(int n, const int64_t* host_table, const eo_adamw_config* confi
   return EO_OK;
 }
 
-size_t eo_grad_norm_scratch_bytes(int n) {
-  if (n < 0) return 0;
-  const size_t tables = static_cast<size_t>(n) / eo::kOptLargeTable + 2;  // two types
-  return sizeof(double) * (tables * 2 * kOptChunks + static_cast<size_t>(n));
+size_t eo_grad_norm_scratch_bytes(int n, int64_t elements) {
+  if (n < 0 || elements < 0) return 0;
+  const int64_t tables = n / eo::kOptLargeTable + 2;  // two types
+  const int64_t most = tables * 2 * kOptChunks, each = elements / eo::kOptTrip;  // chunks, but for the last one of a tensor
+  return sizeof(double) * static_cast<size_t>((each < most ? each : most) + n);
 }
 
 int eo_grad_norm(int n, const int64_t* host_table, float max_norm, int in_place, float* out, void* scratch,
@@ -1017,15 +1018,18 @@ int eo_grad_norm(int n, const int64_t* host_table, float max_norm, int in_place,
   if (int rc = device_setup(&dev)) return rc;
   if (n < 0 || (n > 0 && host_table == nullptr) || out == nullptr)
     return fail(EO_ERR_BAD_ARG, "negative count or null pointer");
-  if (scratch == nullptr || scratch_bytes < eo_grad_norm_scratch_bytes(n))
-    return fail(EO_ERR_WORKSPACE, "grad norm scratch: need %zu bytes, got %zu", eo_grad_norm_scratch_bytes(n), scratch_bytes);
   const int64_t *g = host_table, *numel = g + n, *dtype = numel + n;
   unsigned types = 0;
+  int64_t elements = 0;
   for (int i = 0; i < n; ++i) {
     if (numel[i] < 0 || (numel[i] > 0 && !g[i])) return fail(EO_ERR_BAD_ARG, "tensor %d: null pointer or negative size", i);
     if (dtype[i] != EO_F32 && dtype[i] != EO_BF16) return fail(EO_ERR_BAD_ARG, "tensor %d: gradients are fp32 or bf16", i);
     types |= 1u << dtype[i];
+    elements += numel[i];
   }
+  const size_t need = eo_grad_norm_scratch_bytes(n, elements);
+  if (scratch_bytes < need || (need > 0 && scratch == nullptr))
+    return fail(EO_ERR_WORKSPACE, "grad norm scratch: need %zu bytes, got %zu", need, scratch_bytes);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   double* partials = static_cast<double*>(scratch);
   int64_t used = 0;

@@ -210,7 +210,8 @@ PyObject* adamw_table(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   });
 }
 
-// grads_table(grads, in_place) -> (device, table, types): the three rows of eo_grad_norm and the set (bits) of types in it.
+// grads_table(grads, in_place) -> (device, table, types, elements): the three rows of eo_grad_norm, the set (bits) of types in it
+// and the number of all elements.
 PyObject* grads_table(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   return guarded([&]() -> PyObject* {
     if (nargs != 2) raise(PyExc_TypeError, "grads_table takes 2 arguments");
@@ -221,18 +222,20 @@ PyObject* grads_table(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     const int device = first_device(g);
     std::vector<int64_t> table(3 * n), written;
     unsigned types = 0;
+    long long elements = 0;
     for (int64_t i = 0; i < n; ++i) {
       table[i] = address(g, i, device, kF32 | kBF16, -1);
       table[n + i] = g[i].numel();
       table[2 * n + i] = g[i].scalar_type() == at::kBFloat16 ? 1 : 0;
       types |= 1u << table[2 * n + i];
+      elements += table[n + i];
       if (in_place && table[n + i] > 0) written.push_back(table[i]);
     }
     require_distinct(written, "the gradients");
     if (in_place)
       for (int64_t i = 0; i < n; ++i) mark_written(g[i]);
     Owned bytes(bytes_of(table));
-    return Py_BuildValue("iOI", device, bytes.get(), types);
+    return Py_BuildValue("iOIL", device, bytes.get(), types, elements);
   });
 }
 

@@ -23,8 +23,8 @@ def _norm(grads: Sequence[torch.Tensor], max_norm: float, in_place: bool) -> tor
         raise ValueError(f"max_norm must not be negative, got {max_norm}")
     if not torch.is_tensor(grads):  # a tensor would be taken apart into its rows: the table refuses it
         grads = list(grads)
-    device, table, types = _native.host().grads_table(grads, in_place)
-    return _native.grad_norm(grads, device, table, types, max_norm, in_place)
+    device, table, types, elements = _native.host().grads_table(grads, in_place)
+    return _native.grad_norm(grads, device, table, types, elements, max_norm, in_place)
 
 
 def global_grad_norm(grads: Sequence[torch.Tensor]) -> torch.Tensor:
@@ -38,8 +38,8 @@ def clip_coefficient(grads: Sequence[torch.Tensor], max_norm: float) -> tuple[to
 
     Pass the coefficient to ``AdamW.step(grad_scale=...)``.  A norm that is NaN gives a coefficient that is NaN.
     """
-    norm, coefficient = _norm(grads, max_norm, False).unbind()
-    return norm, coefficient
+    out = _norm(grads, max_norm, False)
+    return out[0], out[1]
 
 
 def clip_grads_(grads: Sequence[torch.Tensor], max_norm: float) -> torch.Tensor:

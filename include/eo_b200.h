@@ -435,9 +435,9 @@ int eo_adamw_step(int n, const int64_t* host_table, const eo_adamw_config* confi
  * (addresses, element counts, EO_F32 / EO_BF16).  Squares are summed in float64 in a fixed order.
  * out[0] = norm, out[1] = min(1, max_norm / (norm + 1e-6)), fp32, in device memory; NaN stays NaN.
  * in_place: the tensors are multiplied by out[1] afterwards (bf16 rounded to nearest even; untouched when it is 1).
- * `scratch`: eo_grad_norm_scratch_bytes(n) bytes, 8-byte aligned.
+ * `scratch`: eo_grad_norm_scratch_bytes(n, elements of all tensors) bytes, 8-byte aligned.
  */
-size_t eo_grad_norm_scratch_bytes(int n);
+size_t eo_grad_norm_scratch_bytes(int n, int64_t elements);
 int eo_grad_norm(int n, const int64_t* host_table, float max_norm, int in_place, float* out, void* scratch,
                  size_t scratch_bytes, void* stream);
 
