@@ -765,7 +765,7 @@ def peek_device_status_async(pinned: torch.Tensor, device: torch.device) -> None
     _check(rc, "eo_peek_device_status_async")
 
 
-# ---- operators over lists of tensors ----------------------------------------------------------------------------------
+# ---- operators over lists of tensors --------------------------------------------------------------------------------
 
 #: Tensors one launch takes, and elements that share an exponent byte of an 8-bit state.
 MAX_TENSORS_PER_LAUNCH = 384
@@ -788,8 +788,8 @@ def host():
             ) from e
         if _host.TORCH_VERSION != torch.__version__.split("+")[0]:
             raise NativeLibraryError(
-                f"the host module was built for torch {_host.TORCH_VERSION}, this is {torch.__version__}: build it again "
-                "with `python -m emerging_optimizers_b200.build --force`"
+                f"the host module was built for torch {_host.TORCH_VERSION}, this is {torch.__version__}: build it "
+                "again with `python -m emerging_optimizers_b200.build --force`"
             )
         _host_module = _host
     return _host_module
@@ -809,8 +809,8 @@ def adamw_step(
     weight_decay: float, method: str, step: int, on_device: bool, state_bits: int, seed: int = 0, first_index: int = 0,
     lr_tensor: torch.Tensor | None = None, grad_scale: torch.Tensor | None = None,
 ) -> None:  # fmt: skip
-    """One AdamW step of the ``n`` tensors of ``table`` (see ``eo_adamw_step``); ``kinds`` is the set of kinds in it, as bits;
-    ``on_device``: the step counters or the learning rate are read from device memory."""
+    """One AdamW step of the ``n`` tensors of ``table`` (see ``eo_adamw_step``); ``kinds`` is the set of kinds in it, as
+    bits; ``on_device``: the step counters or the learning rate are read from device memory."""
     global launch_count
     scratch, scratch_ptr, nbytes = None, 0, 0
     if on_device:
@@ -829,13 +829,13 @@ def adamw_step(
 def grad_norm(
     grads, device: int, table: bytes, types: int, elements: int, max_norm: float, in_place: bool
 ) -> torch.Tensor:
-    """Norm and clipping coefficient of ``grads``, whose ``table`` is (see ``eo_grad_norm``) and whose elements add up to
-    ``elements``, as the first two elements of an fp32 tensor; ``types`` is the set of types in it, as bits; ``in_place`` also
-    multiplies them by the coefficient."""
+    """Norm and clipping coefficient of ``grads``, whose ``table`` is given (see ``eo_grad_norm``) and whose elements add
+    up to ``elements``, as the first two elements of an fp32 tensor; ``types`` is the set of types in it, as bits;
+    ``in_place`` also multiplies them by the coefficient."""
     global launch_count
     n = len(grads)
     nbytes = lib().eo_grad_norm_scratch_bytes(n, elements)
-    # the partial sums of a small set lie behind the result: one allocation less, and little for the result to keep alive
+    # the partial sums of a small set lie behind the result: one allocation less, and little for the result to keep
     apart = nbytes > 8192
     out = grads[0].new_empty(2 if apart else 2 + nbytes // 4, dtype=torch.float32)
     scratch = grads[0].new_empty(nbytes, dtype=torch.uint8) if apart else None
@@ -849,13 +849,16 @@ def grad_norm(
     return out
 
 
-def quantize_blockwise(x: torch.Tensor, signed: bool, seed: int | None, codes: torch.Tensor, exponents: torch.Tensor) -> None:
+def quantize_blockwise(
+    x: torch.Tensor, signed: bool, seed: int | None, codes: torch.Tensor, exponents: torch.Tensor
+) -> None:
     """Codes and exponent bytes of the flat dense tensor ``x``; see ``eo_quantize_blockwise``."""
     global launch_count
     launch_count += 1
     rc = _launch(
         x.get_device(), lib().eo_quantize_blockwise, x.data_ptr(), 1 if x.dtype == torch.bfloat16 else 0, x.numel(),
-        1 if signed else 0, 0 if seed is None else 1, 0 if seed is None else seed, codes.data_ptr(), exponents.data_ptr(),
+        1 if signed else 0, 0 if seed is None else 1, 0 if seed is None else seed, codes.data_ptr(),
+        exponents.data_ptr(),
     )  # fmt: skip
     _check(rc, "eo_quantize_blockwise")
 

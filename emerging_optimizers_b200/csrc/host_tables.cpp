@@ -102,7 +102,8 @@ int64_t address(const Tensors& ts, int64_t i, int device, unsigned types, int64_
   if (!(type_of(t) & types))
     raise(PyExc_TypeError, ts.name() + " must be " + names_of(types) + ", " + ts.at(i) + " is " + c10::toString(t.scalar_type()));
   if (numel >= 0 && t.numel() != numel)
-    raise(PyExc_ValueError, ts.at(i) + " has " + std::to_string(t.numel()) + " elements where " + std::to_string(numel) + " are needed");
+    raise(PyExc_ValueError,
+          ts.at(i) + " has " + std::to_string(t.numel()) + " elements where " + std::to_string(numel) + " are needed");
   if (!t.is_contiguous()) raise(PyExc_ValueError, ts.at(i) + " is not contiguous");
   return reinterpret_cast<int64_t>(t.data_ptr());
 }
@@ -130,7 +131,8 @@ void mark_written(const at::Tensor& t) {
 }
 
 PyObject* bytes_of(const std::vector<int64_t>& table) {
-  return PyBytes_FromStringAndSize(reinterpret_cast<const char*>(table.data()), static_cast<Py_ssize_t>(table.size() * sizeof(int64_t)));
+  const auto bytes = static_cast<Py_ssize_t>(table.size() * sizeof(int64_t));
+  return PyBytes_FromStringAndSize(reinterpret_cast<const char*>(table.data()), bytes);
 }
 
 template <typename F>
@@ -168,7 +170,8 @@ PyObject* adamw_table(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
       column(2)[i] = address(m, i, device, bits8 ? kU8 : kF32, numel);
       column(3)[i] = address(v, i, device, bits8 ? kU8 : kF32, numel);
       column(8)[i] = numel;
-      column(9)[i] = (p[i].scalar_type() == at::kBFloat16 ? 1 : 0) | (g[i].scalar_type() == at::kBFloat16 ? 2 : 0) | (with_remainders ? 4 : 0);
+      column(9)[i] = (p[i].scalar_type() == at::kBFloat16 ? 1 : 0) | (g[i].scalar_type() == at::kBFloat16 ? 2 : 0) |
+                     (with_remainders ? 4 : 0);
       kinds |= 1u << column(9)[i];
       if (numel > 0) written.insert(written.end(), {column(0)[i], column(2)[i], column(3)[i]});
     }
@@ -239,8 +242,8 @@ PyObject* grads_table(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   });
 }
 
-// with_grads(params) -> (those with a gradient, their gradients, whether all of both are contiguous and the parameters of one device
-// and type).
+// with_grads(params) -> (those with a gradient, their gradients, whether all of both are contiguous and the parameters of
+// one device and type).
 PyObject* with_grads(PyObject*, PyObject* arg) {
   return guarded([&]() -> PyObject* {
     Tensors p(arg, "params");
@@ -253,7 +256,8 @@ PyObject* with_grads(PyObject*, PyObject* arg) {
       if (!g.defined()) continue;
       if (g.layout() != at::kStrided) raise(PyExc_RuntimeError, "AdamW does not support sparse gradients");
       if (first == nullptr) first = &t;
-      uniform = uniform && t.is_contiguous() && g.is_contiguous() && t.device() == first->device() && t.scalar_type() == first->scalar_type();
+      uniform = uniform && t.is_contiguous() && g.is_contiguous() && t.device() == first->device() &&
+                t.scalar_type() == first->scalar_type();
       Owned wrapped(THPVariable_Wrap(g));
       if (PyList_Append(params.get(), p.item(i)) != 0 || PyList_Append(grads.get(), wrapped.get()) != 0) throw Raised{};
     }

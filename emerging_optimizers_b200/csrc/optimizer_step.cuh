@@ -324,7 +324,8 @@ struct Code8 {
     }
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
-      uint32_t w = __byte_perm(__byte_perm(t[4 * j], t[4 * j + 1], 0x0073), __byte_perm(t[4 * j + 2], t[4 * j + 3], 0x0073), 0x5410);
+      uint32_t w = __byte_perm(__byte_perm(t[4 * j], t[4 * j + 1], 0x0073),
+                               __byte_perm(t[4 * j + 2], t[4 * j + 3], 0x0073), 0x5410);
       if constexpr (kSigned) {
         const uint32_t signs = __byte_perm(
             __byte_perm(__float_as_uint(x[4 * j]), __float_as_uint(x[4 * j + 1]), 0x0073),

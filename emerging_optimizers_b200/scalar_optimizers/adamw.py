@@ -1,8 +1,8 @@
 """AdamW over many tensors at once, with moments in fp32 or in 8 bits.
 
 The scalar optimizer that a model's embeddings, output layer and 1-D parameters need beside the orthogonalized ones
-(the reference keeps its scalar optimizers in ``emerging_optimizers/scalar_optimizers``).  A step of a parameter group is
-one launch for each mix of types (up to 384 tensors), whatever their sizes.
+(the reference keeps its scalar optimizers in ``emerging_optimizers/scalar_optimizers``).  A step of a parameter group
+is one launch for each mix of types (up to 384 tensors), whatever their sizes.
 """
 
 from __future__ import annotations
@@ -67,7 +67,9 @@ def _step(
         params, grads, m, v, m_exponents, v_exponents, remainders, None if on_host else step
     )
     if on_host and host.stream(device)[2]:
-        raise RuntimeError("a step number given as an int would be frozen into the captured graph: pass an int64 device tensor")
+        raise RuntimeError(
+            "a step number given as an int would be frozen into the captured graph: pass an int64 device tensor"
+        )
     lr_tensor = None
     if torch.is_tensor(lr):
         if lr.is_cuda:
@@ -239,7 +241,7 @@ class AdamW(optim.Optimizer):
         state = self.state.get(p)
         if not state:
             raise ValueError("the parameter has no state yet")
-        return tuple(self._values(state, name, signed) for name, signed in (("exp_avg", True), ("exp_avg_sq", False)))  # type: ignore[return-value]
+        return self._values(state, "exp_avg", True), self._values(state, "exp_avg_sq", False)
 
     @staticmethod
     def _values(state: dict, name: str, signed: bool) -> torch.Tensor:
@@ -268,7 +270,9 @@ class AdamW(optim.Optimizer):
                 for p, state in zip(params, states):
                     if not state:
                         if p.is_cuda and torch.cuda.is_current_stream_capturing():
-                            raise RuntimeError("run a step before capturing one: the state must exist when the capture begins")
+                            raise RuntimeError(
+                                "run a step before capturing one: the state must exist when the capture begins"
+                            )
                         state.update(self._new_state(p))
             # one call per device, type of parameter and step number (with device counters: whatever the number)
             steps = [0] * len(params) if self.capturable else [state["step"] + 1 for state in states]
@@ -282,7 +286,11 @@ class AdamW(optim.Optimizer):
                 first_index += self._call(group, *lists, uniform, call[2], grad_scale, first_index)
         return None
 
-    def _call(self, group, params, grads, states, plain, step, grad_scale, first_index) -> int:  # type: ignore[no-untyped-def]
+    def _call(  # type: ignore[no-untyped-def]
+        self, group, params, grads, states, plain, step, grad_scale, first_index
+    ) -> int:
+        """The step of parameters of one device, type and step number; ``plain``: all of them and their gradients are
+        contiguous.  Returns their number."""
         if not plain:
             orders = [_memory_order(p) for p in params]
             grads = [_flat(g, o) for g, o in zip(grads, orders)]
@@ -354,7 +362,8 @@ class AdamW(optim.Optimizer):
                 x = self._values({name: x, exponents: saved[exponents].to(p.device)}, name, signed)
             if self.state_bits == 8:
                 order = _memory_order(p)
-                codes, state[exponents] = quantize_blockwise(_flat(torch.empty_like(p, dtype=torch.float32).copy_(x), order), signed=signed)
+                values = torch.empty_like(p, dtype=torch.float32).copy_(x)
+                codes, state[exponents] = quantize_blockwise(_flat(values, order), signed=signed)
                 _flat(state[name], order).copy_(codes)
             else:
                 state[name].copy_(x)

@@ -1,8 +1,8 @@
 """8-bit block-scaled numbers: the format of ``AdamW(state_bits=8)``'s moments.
 
 Every 256 consecutive elements (in memory order) share one exponent byte, the fp32 exponent field of their largest
-finite magnitude.  A code is a small float below that power of two: signed numbers have a sign, 4 exponent and 3 mantissa
-bits, unsigned ones 5 exponent and 3 mantissa bits.  What is not finite (unsigned: or is negative) reads back as NaN; an
+finite magnitude.  A code is a small float below that power of two: signed numbers have a sign, 4 exponent and 3
+mantissa bits, unsigned ones 5 exponent and 3 mantissa bits.  What is not finite (unsigned: or is negative) reads back as NaN; an
 unsigned number above zero never becomes zero.
 """
 

@@ -2,7 +2,8 @@
 
 The clipping coefficient stays on the device: :func:`clip_coefficient` hands it to
 ``AdamW.step(grad_scale=...)``, which then scales the gradients as it reads them, so that they are read once for the
-norm and never written back.  :func:`clip_grads_` / :func:`clip_grad_norm_` scale them in place for every other consumer.
+norm and never written back.  :func:`clip_grads_` / :func:`clip_grad_norm_` scale them in place for every other
+consumer.
 """
 
 from __future__ import annotations
@@ -34,7 +35,8 @@ def global_grad_norm(grads: Sequence[torch.Tensor]) -> torch.Tensor:
 
 
 def clip_coefficient(grads: Sequence[torch.Tensor], max_norm: float) -> tuple[torch.Tensor, torch.Tensor]:
-    """``(norm, min(1, max_norm / (norm + 1e-6)))`` as fp32 scalar tensors on the device; the gradients stay as they are.
+    """``(norm, min(1, max_norm / (norm + 1e-6)))`` as fp32 scalar tensors on the device; the gradients stay as they
+    are.
 
     Pass the coefficient to ``AdamW.step(grad_scale=...)``.  A norm that is NaN gives a coefficient that is NaN.
     """

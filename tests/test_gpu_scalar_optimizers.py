@@ -97,8 +97,9 @@ def test_adamw_step_gives_the_bits_of_single_operations(method, steps):
     p0, m0, v0 = p.clone(), m.clone(), v.clone()
     lr, (b1, b2), eps, wd = HYPER["lr"], HYPER["betas"], HYPER["eps"], HYPER["weight_decay"]
     for step in steps:
-        adamw_step([p], [g], [m], [v], **HYPER, step=step, weight_decay_method=method, grad_scale=torch.tensor(0.7, device="cuda"))
-        x = g * torch.tensor(0.7, device="cuda")
+        scale = torch.tensor(0.7, device="cuda")
+        adamw_step([p], [g], [m], [v], **HYPER, step=step, weight_decay_method=method, grad_scale=scale)
+        x = g * scale
         if method == "l2":
             x = x + p0 * wd
         p0 = p0 * ref.decay_factor(method, lr, wd)
@@ -462,7 +463,7 @@ def test_norms_that_are_not_finite():
 
 
 def test_clip_grad_norm_matches_torch():
-    params = [torch.nn.Parameter(torch.zeros(n, device="cuda")) for n in (10, 1000, 33)] + [torch.nn.Parameter(torch.zeros(4, device="cuda"))]
+    params = [torch.nn.Parameter(torch.zeros(n, device="cuda")) for n in (10, 1000, 33, 4)]
     other = [torch.nn.Parameter(torch.zeros_like(p)) for p in params]
     for i, (p, q) in enumerate(zip(params[:3], other)):
         p.grad, q.grad = _randn(p.numel(), i), _randn(p.numel(), i)
@@ -488,10 +489,10 @@ def _set_grads(params, step, dtype=None):
 
 def test_optimizer_matches_torch_adamw():
     a, b = _model_params(), _model_params()
-    ours = AdamW([{"params": a[:2], "lr": 1e-2}, {"params": a[2:], "weight_decay": 0.0}], lr=3e-3, betas=(0.9, 0.99), weight_decay=0.1)
-    theirs = torch.optim.AdamW(
-        [{"params": b[:2], "lr": 1e-2}, {"params": b[2:], "weight_decay": 0.0}], lr=3e-3, betas=(0.9, 0.99), weight_decay=0.1
-    )
+    ours, theirs = [
+        cls([{"params": x[:2], "lr": 1e-2}, {"params": x[2:], "weight_decay": 0.0}], lr=3e-3, betas=(0.9, 0.99), weight_decay=0.1)
+        for cls, x in ((AdamW, a), (torch.optim.AdamW, b))
+    ]  # fmt: skip
     schedules = [torch.optim.lr_scheduler.ExponentialLR(o, 0.9) for o in (ours, theirs)]
     for step in range(6):
         _set_grads(a, step)
@@ -522,8 +523,8 @@ def test_checkpoint_resumes_bit_for_bit(bits, dtype):
         if step == 2:
             b = [torch.nn.Parameter(p.detach().clone()) for p in a]
             saved = whole.state_dict()
-            saved = {"state": {i: {k: v.cpu() if torch.is_tensor(v) else v for k, v in s.items()} for i, s in saved["state"].items()},
-                     "param_groups": saved["param_groups"]}  # fmt: skip
+            for i, state in saved["state"].items():  # as it comes back from a file
+                saved["state"][i] = {k: v.cpu() if torch.is_tensor(v) else v for k, v in state.items()}
             rest = AdamW(b, **kw)
             rest.load_state_dict(saved)
         for params, opt in ((a, whole),) + (((b, rest),) if step >= 2 else ()):
@@ -727,7 +728,8 @@ def test_many_calls_queued_without_waiting():
 
 
 def test_zero_dimensional_and_empty_parameters():
-    params = [torch.nn.Parameter(t) for t in (torch.tensor(2.0, device="cuda"), torch.empty(0, 3, device="cuda"), torch.ones(1, 1, device="cuda"))]
+    values = (torch.tensor(2.0, device="cuda"), torch.empty(0, 3, device="cuda"), torch.ones(1, 1, device="cuda"))
+    params = [torch.nn.Parameter(t) for t in values]
     for bits in (32, 8):
         opt = AdamW(params, lr=0.1, weight_decay=0.0, state_bits=bits)
         for p in params:
@@ -836,7 +838,8 @@ def test_refusals_on_the_gpu():
 def test_muon_and_adamw_train_one_model_together():
     """Matrices by Muon, the rest by AdamW with 8-bit moments, one global norm over both: the calls a training loop makes."""
     torch.manual_seed(0)
-    model = torch.nn.Sequential(torch.nn.Embedding(100, 64), torch.nn.Linear(64, 128), torch.nn.LayerNorm(128), torch.nn.Linear(128, 100)).cuda()
+    layers = torch.nn.Embedding(100, 64), torch.nn.Linear(64, 128), torch.nn.LayerNorm(128), torch.nn.Linear(128, 100)
+    model = torch.nn.Sequential(*layers).cuda()
     hidden = [model[1].weight]
     rest = [p for p in model.parameters() if p is not hidden[0]]
     muon = Muon(hidden, lr=0.01)
