@@ -171,7 +171,7 @@ def _flat(t: torch.Tensor, order: tuple[int, ...] | None) -> torch.Tensor:
     return (t if order is None else t.permute(order)).contiguous()
 
 
-@registry.register_optimizer("adamw")
+@registry.register_optimizer("fused_adamw")
 class AdamW(optim.Optimizer):
     """AdamW whose step takes all tensors of a group in one launch.
 

@@ -37,9 +37,9 @@ def test_adamw_refuses_bad_hyperparameters(kw):
 
 
 def test_adamw_is_registered_and_checks_names():
-    assert registry.get_optimizer_cls("adamw") is AdamW
+    assert registry.get_optimizer_cls("fused_adamw") is AdamW
     with pytest.raises(TypeError):
-        registry.get_configured_optimizer_cls("adamw", momentum=0.9)
+        registry.get_configured_optimizer_cls("fused_adamw", momentum=0.9)
 
 
 def test_cpu_tensors_are_refused():
