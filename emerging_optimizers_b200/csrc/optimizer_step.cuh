@@ -204,7 +204,8 @@ __device__ __forceinline__ void split_masters(const float2 (&x)[4], Run<__nv_bfl
 // a small float, its bits those of an fp32 number shifted right by 20:
 //   signed   (first moments):  sign, 4 exponent bits, 3 mantissa bits; down to 2^-16 of the block's power of two
 //   unsigned (second moments):       5 exponent bits, 3 mantissa bits; down to 2^-32
-//   value = f32(code << 20) * 2^kShift * 2^(E - 127),    code = (bits(|x| * 2^(127 - E) * 2^-kShift) + d) >> 20
+//   value = f32(code << 20) * 2^kShift * 2^(E - 127),    code = (bits(|x| * 2^(127 - E) * 2^-kShift) + d) >> 20,
+//   kShift = 113 and 97,
 // so the block's largest magnitude has exponent field 14 (of 15) or 30 (of 31): rounding up never leaves the format, and
 // values lie exactly in bf16 and fp32 because the scale is a power of two.  The second moment itself is stored, not its
 // root: decoding needs no multiplication and rounding is unbiased in what the moving average averages.
@@ -229,9 +230,7 @@ template <bool kSigned>
 struct Code8 {
   static constexpr int kTop = kSigned ? 14 : 30;
   static constexpr uint32_t kNan = kSigned ? 0x7f : 0xff;
-  // 2^kShift and 2^-kShift with kShift = 127 - kTop
-  static __device__ __forceinline__ float up() { return __uint_as_float(static_cast<uint32_t>(254 - kTop) << 23); }
-  static __device__ __forceinline__ float down() { return __uint_as_float(static_cast<uint32_t>(kTop) << 23); }
+  static __device__ __forceinline__ float down() { return __uint_as_float(static_cast<uint32_t>(kTop) << 23); }  // 2^-kShift
 
   static __device__ __forceinline__ void decode(const Run<uint8_t>& codes, uint32_t exponent, float2 (&out)[4]) {
     if constexpr (kSigned) {
@@ -245,14 +244,19 @@ struct Code8 {
         out[k] = mul2(__half22float2(*reinterpret_cast<const __half2*>(&h2)), scale);
       }
     } else {
-      const float2 scale = both(__uint_as_float(exponent << 23)), lift = both(up());
+      // 2^97 * 2^(E - 127), in two steps where it leaves the fp32 range
+      const float2 scale = both(__uint_as_float((min(exponent, 157u) + 97u) << 23));
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         const uint32_t w = codes.w[k / 2];
         // the byte at bit 16, times 2^4
         const uint32_t a = __byte_perm(w, 0, 0x4044 | (2 * (k % 2)) << 8) * 16u;
         const uint32_t b = __byte_perm(w, 0, 0x4044 | (2 * (k % 2) + 1) << 8) * 16u;
-        out[k] = mul2(mul2(make_float2(__uint_as_float(a), __uint_as_float(b)), lift), scale);
+        out[k] = mul2(make_float2(__uint_as_float(a), __uint_as_float(b)), scale);
+      }
+      if (exponent > 157u) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) out[k] = mul2(out[k], both(__uint_as_float((exponent - 30u) << 23)));
       }
       const uint32_t nans = ((~codes.w[0] - 0x01010101u) & codes.w[0]) | ((~codes.w[1] - 0x01010101u) & codes.w[1]);
       if (nans & 0x80808080u) {  // a byte is 0xff
@@ -288,7 +292,8 @@ struct Code8 {
   static __device__ __forceinline__ uint32_t quantize(const float2 (&in)[4], const uint32_t (&d16)[8], Run<uint8_t>& codes) {
     const float x[8] = {in[0].x, in[0].y, in[1].x, in[1].y, in[2].x, in[2].y, in[3].x, in[3].y};
     uint32_t top = block_top(x);
-    const bool rare = top >= 0x7f000000u;  // 2^127 and beyond, infinity, NaN; unsigned: a negative number
+    // Beyond what one factor reaches (2^14 for first, 2^30 for second moments), infinity, NaN; unsigned: a negative number.
+    const bool rare = top >= static_cast<uint32_t>(127 + kTop) << 23;
     if (rare) {
       uint32_t mine = 0;
 #pragma unroll
@@ -297,13 +302,12 @@ struct Code8 {
       top = __reduce_max_sync(0xffffffffu, mine);
     }
     const uint32_t e = max(top >> 23, 1u);
-    // 2^(127 - e); subnormal for e = 254
-    const float2 inv = both(__uint_as_float(max((254u - e) << 23, 0x00400000u))), lower = both(down());
+    const float2 factor = both(__uint_as_float((127u + kTop - e) << 23));  // 2^(127 - E) * 2^-kShift
     uint32_t t[8];
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
       // 16 (bits + d) has the code in its top byte; the sign, if any, is shifted out
-      const float2 y = mul2(mul2(in[k], inv), lower);
+      const float2 y = mul2(in[k], factor);
       t[2 * k] = __float_as_uint(y.x) * 16u + d16[2 * k];
       t[2 * k + 1] = __float_as_uint(y.y) * 16u + d16[2 * k + 1];
       if constexpr (!kSigned) {
@@ -312,14 +316,13 @@ struct Code8 {
       }
     }
     if (rare) {
+      const float inv = __uint_as_float(max((254u - e) << 23, 0x00400000u));  // 2^(127 - e); subnormal for e = 254
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
-        const float v = k % 2 == 0 ? in[k / 2].x : in[k / 2].y;
-        if (e == 254u) {  // towards zero: without d
-          t[k] -= d16[k];
-          if (!kSigned && v > 0.0f) t[k] = max(__float_as_uint(__fmul_rn(__fmul_rn(v, inv.x), lower.x)) * 16u, 1u << 24);
-        }
-        if (!is_kept(v)) t[k] = (!kSigned && __float_as_uint(v) == 0x80000000u) ? 0u : kNan << 24;  // -0 is kept as 0
+        const float y = __fmul_rn(__fmul_rn(x[k], inv), down());
+        t[k] = __float_as_uint(y) * 16u + (e == 254u ? 0u : d16[k]);  // towards zero in the last binade
+        if (!kSigned && x[k] > 0.0f) t[k] = max(t[k], 1u << 24);
+        if (!is_kept(x[k])) t[k] = (!kSigned && __float_as_uint(x[k]) == 0x80000000u) ? 0u : kNan << 24;  // -0 is kept as 0
       }
     }
 #pragma unroll

@@ -373,6 +373,23 @@ def test_quantizer_gives_the_codes_of_its_statement(signed, dtype, n, seed):
 
 
 @pytest.mark.parametrize("signed", [True, False])
+@pytest.mark.parametrize("seed", [None, 7])
+def test_quantizer_at_every_block_exponent(signed, seed):
+    """One block for every power of two of the fp32 range, values down to 2^-35 of it."""
+    rng = np.random.default_rng(5)
+    rows = [np.ldexp(rng.uniform(1, 2, 256) * np.ldexp(1.0, -rng.integers(0, 36, 256)), e) for e in range(-130, 128)]
+    x = np.concatenate(rows).astype(np.float32)
+    x = np.where(rng.random(x.size) < 0.5, -x, x) if signed else x
+    codes, exponents = quantize_blockwise(torch.from_numpy(x).cuda(), signed=signed, seed=seed)
+    bits = None if seed is None else ref.random_bits(x.size, seed, 0, 0, signed)
+    want, want_e = ref.quantize(x, signed, bits)
+    assert np.array_equal(exponents.cpu().numpy(), want_e)
+    assert np.array_equal(codes.cpu().numpy(), want)
+    y = dequantize_blockwise(codes, exponents, signed=signed)
+    assert np.array_equal(_np64(y), ref.dequantize(want, want_e, signed).astype(np.float32).astype(np.float64))
+
+
+@pytest.mark.parametrize("signed", [True, False])
 def test_quantizer_at_the_ends_of_the_fp32_range(signed):
     tiny, huge = 2.0**-126, 3.4e38
     rows = [
