@@ -569,7 +569,7 @@ struct AdamWCursor {
 };
 
 // Runs of the 8-bit step on their way through shared memory: a warp's own ring of kRingStages runs, filled by asynchronous
-// copies two trips ahead.  Without it the loads wait for the 60 instructions an element that lie between a load and its
+// copies two trips ahead.  Without it the loads wait for the 59 instructions an element that lie between a load and its
 // store, and prefetching into registers costs the occupancy it should replace: 268 M fp32 elements 1028 us without, 650 us
 // with the ring.  Three stages leave room for three CTAs an SM with fp32 types; four (two CTAs) are 4 % slower under a
 // sustained load, two 3 % slower with bf16 gradients.
@@ -635,11 +635,11 @@ struct AdamWRing {
 
 // kRemainder: p is bf16 with remainders.  k8: m and v are codes with exponent bytes.
 // fp32 moments: bound by HBM.  268 M elements: fp32 types 1.13 ms (28 bytes an element, 6.65 TB/s), bf16 gradients 1.06 ms
-// (6.6), bf16 0.92 ms (6.4), bf16 with remainders 1.09 ms (6.4).
-// 8-bit moments: 60 instructions an element for its 10 to 16 bytes.  fp32 types 0.65 ms (6.6 TB/s), bf16 gradients 0.59 ms (6.3),
-// bf16 with remainders 0.65 ms (5.8) and bf16 0.63 ms (4.3): the last is bound by the issue slots (78 % used, the integer
+// (6.6), bf16 0.91 ms (6.5), bf16 with remainders 1.09 ms (6.4).
+// 8-bit moments: 59 instructions an element for its 10 to 16 bytes.  fp32 types 0.65 ms (6.6 TB/s), bf16 gradients 0.58 ms (6.5),
+// bf16 with remainders 0.64 ms (5.8) and bf16 0.58 ms (4.6): the last is bound by the issue slots (78 % used, the integer
 // multiply pipe 73 %).  These are bursts; run without a pause the 8-bit step reaches the GPU's power limit and its clock falls
-// from 1.97 to 1.6 GHz (fp32 types 0.74 ms), the others do not slow down.
+// from 1.97 to 1.6 GHz (fp32 types 0.73 ms, bf16 0.59), while the step with fp32 moments does not slow down.
 // Three CTAs an SM (80 registers): two are 6 - 12 % slower with bf16 types, four spill.
 template <typename P, typename G, bool kRemainder, bool k8, int kCapacity>
 __global__ void __launch_bounds__(kOptThreads, 3)
