@@ -105,6 +105,7 @@ int64_t address(const Tensors& ts, int64_t i, int device, unsigned types, int64_
     raise(PyExc_ValueError,
           ts.at(i) + " has " + std::to_string(t.numel()) + " elements where " + std::to_string(numel) + " are needed");
   if (!t.is_contiguous()) raise(PyExc_ValueError, ts.at(i) + " is not contiguous");
+  if (t.is_neg()) raise(PyExc_ValueError, ts.at(i) + " is a negated view");
   return reinterpret_cast<int64_t>(t.data_ptr());
 }
 

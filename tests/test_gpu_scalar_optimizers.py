@@ -625,9 +625,10 @@ def test_parameters_in_other_memory_orders(bits):
 
 
 @pytest.mark.parametrize("bits", [32, 8])
-def test_captured_step_replays_as_eager_steps(bits):
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_captured_step_replays_as_eager_steps(bits, dtype):
     kw = dict(betas=(0.9, 0.99), weight_decay=0.1, state_bits=bits, capturable=True, seed=3)
-    a, b = _model_params(BF16), _model_params(BF16)
+    a, b = _model_params(dtype), _model_params(dtype)
     lrs = [torch.tensor(1e-2, device="cuda") for _ in range(2)]
     eager, graphed = AdamW(a, lr=lrs[0], **kw), AdamW(b, lr=lrs[1], **kw)
     _set_grads(a, 0)

@@ -64,6 +64,23 @@ def test_cpu_tensors_are_refused():
     assert torch.equal(p.detach(), torch.ones(5))
 
 
+def test_host_module_of_another_torch_is_refused(monkeypatch):
+    monkeypatch.setattr(_native, "_host_module", None)
+    monkeypatch.setattr(torch, "__version__", "9.9.9")
+    with pytest.raises(_native.NativeLibraryError, match="built for torch"):
+        _native.host()
+
+
+def test_scratch_queries_need_no_gpu():
+    lib = _native.lib()
+    assert lib.eo_adamw_scratch_bytes(0) == 0 and lib.eo_adamw_scratch_bytes(7) == 7 * 16
+    small = lib.eo_grad_norm_scratch_bytes(3, 5000)
+    assert small >= 8 * (3 + 2)  # a partial sum for every begun chunk of 2048 elements
+    assert lib.eo_grad_norm_scratch_bytes(-1, 5) == 0
+    huge = lib.eo_grad_norm_scratch_bytes(1, 1 << 40)
+    assert small < huge < 1 << 20  # the number of chunks is bounded
+
+
 def test_other_refusals_that_need_no_gpu():
     p = _p(5)
     p.grad = torch.ones(5)
