@@ -181,11 +181,22 @@ __device__ __forceinline__ float2 product(float2 a, float2 b, float2 minus_zero)
 // bf16 weights whose fp32 master is kept as bf16 plus a signed 16-bit remainder: master bits = (bf16 bits << 16) +
 // remainder.  Written back as the nearest bf16 (halves away from zero, so that the remainder fits 16 bits); a NaN
 // becomes the quiet NaN with remainder zero, as adding to its payload could wrap.
+// A weight that somebody set to zero since (a mask, a padding row) may still have a negative remainder, which no split leaves beside
+// a zero and which would borrow from the sign: it is zero then.
 __device__ __forceinline__ void join_masters(const Run<__nv_bfloat16>& hi, const Run<int16_t>& lo, float2 (&out)[4]) {
+  uint32_t zeros = 0;
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
+    zeros |= ((hi.w[k] & 0x7fff7fffu) - 0x00010001u) & 0x80008000u;
     out[k].x = __uint_as_float((hi.w[k] << 16) + static_cast<uint32_t>(static_cast<int32_t>(lo.w[k] << 16) >> 16));
     out[k].y = __uint_as_float((hi.w[k] & 0xffff0000u) + static_cast<uint32_t>(static_cast<int32_t>(lo.w[k]) >> 16));
+  }
+  if (zeros != 0) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      if ((hi.w[k] & 0x7fffu) == 0 && (lo.w[k] & 0x8000u)) out[k].x = 0.0f;
+      if ((hi.w[k] & 0x7fff0000u) == 0 && (lo.w[k] & 0x80000000u)) out[k].y = 0.0f;
+    }
   }
 }
 __device__ __forceinline__ void split_masters(const float2 (&x)[4], Run<__nv_bfloat16>& hi, Run<int16_t>& lo) {

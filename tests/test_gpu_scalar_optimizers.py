@@ -212,6 +212,25 @@ def test_remainders_of_special_values():
 
 
 @pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("n", [5, 2048])
+def test_weights_set_to_zero_with_stale_remainders(bits, n):
+    """A mask or a padding row zeroes bf16 weights and leaves their remainders: they count as zeros (a remainder that is not
+    negative as the subnormal number that it stands for)."""
+    (p,), (g,), (m,), (v,) = _inputs([n], BF16, BF16)
+    r = torch.arange(n, device="cuda").sub(n // 2).to(torch.int16)
+    p[::2] = torch.where(torch.arange(0, n, 2, device="cuda") % 4 == 0, 0.0, -0.0).bfloat16()
+    fresh, r_fresh = p.clone(), r.clone()
+    r_fresh[(p == 0) & (r < 0)] = 0
+    for q, rem in ((p, r), (fresh, r_fresh)):
+        if bits == 32:
+            adamw_step([q], [g], [m.clone()], [v.clone()], **HYPER, step=3, remainders=[rem])
+        else:
+            state = [[t] for t in (*quantize_blockwise(m, signed=True), *quantize_blockwise(v, signed=False))]
+            adamw_step_8bit([q], [g], *state, **HYPER, step=3, seed=1, remainders=[rem])
+    assert bool(torch.isfinite(p).all()) and _same(p, fresh) and torch.equal(r, r_fresh)
+
+
+@pytest.mark.parametrize("bits", [32, 8])
 def test_values_that_are_not_finite_stay_where_they_are(bits):
     n = 1000
     (p,), (g,), (m,), (v,) = _inputs([n])
