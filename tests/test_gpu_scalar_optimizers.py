@@ -1,10 +1,13 @@
 """AdamW with 32- and 8-bit moments, gradient norm and clipping, and the block quantiser on the GPU, against their
 float64 statements."""
 
+import os
+
 import numpy as np
 import pytest
 import torch
 
+from emerging_optimizers_b200 import build as eo_build
 from emerging_optimizers_b200 import utils
 from emerging_optimizers_b200.orthogonalized_optimizers import Muon
 from emerging_optimizers_b200.scalar_optimizers import (
@@ -24,6 +27,12 @@ ULP = 2.0**-24  # one fp32 rounding, relative
 SIZES = [1, 255, 256, 257, 0, 2048, 2049, 12345]
 HYPER = dict(lr=3e-3, betas=(0.9, 0.95), eps=1e-8, weight_decay=0.1)
 REF = dict(lr=3e-3, betas=(0.9, 0.95), eps=1e-8, wd=0.1)
+
+
+@pytest.fixture(scope="module", autouse=True)
+def host_module():
+    if not os.path.exists(eo_build.HOST_OUT):
+        eo_build.build_host()
 
 
 def _randn(n, seed, scale=1.0):
