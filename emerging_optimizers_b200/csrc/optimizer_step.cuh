@@ -282,7 +282,8 @@ struct Code8 {
   }
 
   // Largest magnitude of the block as fp32 bits; at least those of infinity where something is not a number to be kept.
-  static __device__ __forceinline__ uint32_t block_top(const float (&x)[8]) {
+  static __device__ __forceinline__ uint32_t block_top(const float2 (&in)[4]) {
+    const float x[8] = {in[0].x, in[0].y, in[1].x, in[1].y, in[2].x, in[2].y, in[3].x, in[3].y};
     uint32_t top;
     if constexpr (kSigned) {
       const float a = max3_nan(fabsf(x[0]), fabsf(x[1]), fabsf(x[2])), b = max3_nan(fabsf(x[3]), fabsf(x[4]), fabsf(x[5]));
@@ -299,13 +300,17 @@ struct Code8 {
     return (kSigned ? (b & 0x7fffffffu) : b) < 0x7f800000u;
   }
 
-  // Exponent byte and codes of a block; d16[k]: 16 d of each element.
-  static __device__ __forceinline__ uint32_t quantize(const float2 (&in)[4], const uint32_t (&d16)[8], Run<uint8_t>& codes) {
+  // Whether a block with this top takes the rare path: beyond what one factor reaches (2^14 for first, 2^30 for second moments),
+  // infinity, NaN; unsigned: a negative number.
+  static __device__ __forceinline__ bool is_rare(uint32_t top) { return top >= static_cast<uint32_t>(127 + kTop) << 23; }
+
+  // Exponent byte and codes of a block; d16[k]: 16 d of each element; top: of block_top.  kRare is right for every block, the other
+  // one where is_rare(top) is false.
+  template <bool kRare>
+  static __device__ __forceinline__ uint32_t encode(const float2 (&in)[4], uint32_t top, const uint32_t (&d16)[8],
+                                                    Run<uint8_t>& codes) {
     const float x[8] = {in[0].x, in[0].y, in[1].x, in[1].y, in[2].x, in[2].y, in[3].x, in[3].y};
-    uint32_t top = block_top(x);
-    // Beyond what one factor reaches (2^14 for first, 2^30 for second moments), infinity, NaN; unsigned: a negative number.
-    const bool rare = top >= static_cast<uint32_t>(127 + kTop) << 23;
-    if (rare) {
+    if constexpr (kRare) {
       uint32_t mine = 0;
 #pragma unroll
       for (int k = 0; k < 8; ++k)
@@ -313,20 +318,8 @@ struct Code8 {
       top = __reduce_max_sync(0xffffffffu, mine);
     }
     const uint32_t e = max(top >> 23, 1u);
-    const float2 factor = both(__uint_as_float((127u + kTop - e) << 23));  // 2^(127 - E) * 2^-kShift
-    uint32_t t[8];
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      // 16 (bits + d) has the code in its top byte; the sign, if any, is shifted out
-      const float2 y = mul2(in[k], factor);
-      t[2 * k] = __float_as_uint(y.x) * 16u + d16[2 * k];
-      t[2 * k + 1] = __float_as_uint(y.y) * 16u + d16[2 * k + 1];
-      if constexpr (!kSigned) {
-        if (in[k].x > 0.0f) t[2 * k] = max(t[2 * k], 1u << 24);
-        if (in[k].y > 0.0f) t[2 * k + 1] = max(t[2 * k + 1], 1u << 24);
-      }
-    }
-    if (rare) {
+    uint32_t t[8];  // 16 (bits + d) has the code in its top byte; the sign, if any, is shifted out
+    if constexpr (kRare) {
       const float inv = __uint_as_float(max((254u - e) << 23, 0x00400000u));  // 2^(127 - e); subnormal for e = 254
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
@@ -334,6 +327,18 @@ struct Code8 {
         t[k] = __float_as_uint(y) * 16u + (e == 254u ? 0u : d16[k]);  // towards zero in the last binade
         if (!kSigned && x[k] > 0.0f) t[k] = max(t[k], 1u << 24);
         if (!is_kept(x[k])) t[k] = (!kSigned && __float_as_uint(x[k]) == 0x80000000u) ? 0u : kNan << 24;  // -0 is kept as 0
+      }
+    } else {
+      const float2 factor = both(__uint_as_float((127u + kTop - e) << 23));  // 2^(127 - E) * 2^-kShift
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const float2 y = mul2(in[k], factor);
+        t[2 * k] = __float_as_uint(y.x) * 16u + d16[2 * k];
+        t[2 * k + 1] = __float_as_uint(y.y) * 16u + d16[2 * k + 1];
+        if constexpr (!kSigned) {
+          if (in[k].x > 0.0f) t[2 * k] = max(t[2 * k], 1u << 24);
+          if (in[k].y > 0.0f) t[2 * k + 1] = max(t[2 * k + 1], 1u << 24);
+        }
       }
     }
 #pragma unroll
@@ -463,11 +468,6 @@ __device__ __forceinline__ float rcp_approx(float x) {
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-__device__ __forceinline__ float at_least(float x, float low) {  // NaN stays NaN
-  float y;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(x), "f"(low));
-  return y;
-}
 
 // g, p, m, v of one lane, two elements to an instruction.  Every operation is rounded once, in this order, so that the result
 // does not depend on how the compiler would contract it (the 8-bit codes of a run must not depend on the build).
@@ -478,34 +478,59 @@ __device__ __forceinline__ float at_least(float x, float low) {  // NaN stays Na
 // same where the operand is at least 2^-102; with __fdiv_rn on 3.4e10 pairs of mantissas: the same, and the reciprocal inside is
 // the nearest for every mantissa.  Below 2^-102 a root does not count beside an eps of 1e-10 and more.  Where eps is smaller the
 // root is taken of 2^36 v: right within three roundings down to the smallest subnormal v (the 2^-126 that keeps the
-// approximation of zero finite is 2^-13 of it then, and the Newton step squares that), and what lies above 2^92 counts as
-// the largest finite number, as infinity does otherwise.  Zero gives zero.  Negated operands (-v, -root, -denominator) save the
-// sign changes that the paired instructions do not have.
-__device__ __forceinline__ void adamw_update(float2 (&p)[4], const float2 (&g_in)[4], float2 (&m)[4], float2 (&v)[4],
-                                             const AdamWScalars& c, const AdamWFactors& f, float grad_scale) {
+// approximation of zero finite is 2^-13 of it then, and the Newton step squares that).  Zero gives zero.  Negated operands (-v,
+// -root, -denominator) save the sign changes that the paired instructions do not have.
+__device__ __forceinline__ float2 adamw_quotient(float2 m, float2 v, float root_scale, float2 inv, float2 minus_eps, float2 mz) {
+  const float2 nv = mul2(v, both(root_scale));
+  const float2 above_zero = add2(nv, both(-0x1p-126f));
+  const float2 y = make_float2(rsqrt_approx(-above_zero.x), rsqrt_approx(-above_zero.y));
+  float2 nroot = product(nv, y, mz);
+  nroot = fma2(fma2(nroot, nroot, nv), mul2(y, both(0.5f)), nroot);
+  const float2 nd = add2(product(nroot, inv, mz), minus_eps);
+  float2 z = make_float2(rcp_approx(-nd.x), rcp_approx(-nd.y));
+  z = fma2(z, fma2(nd, z, both(1.0f)), z);
+  const float2 q = product(m, z, mz);
+  return fma2(fma2(nd, q, m), z, q);
+}
+
+__device__ __forceinline__ void adamw_moments(const float2 (&p)[4], const float2 (&g_in)[4], float2 (&m)[4], float2 (&v)[4],
+                                              const AdamWScalars& c, float grad_scale) {
   const float2 scale = both(grad_scale), b1 = both(c.beta1), ob1 = both(c.one_minus_beta1), b2 = both(c.beta2);
-  const float2 ob2 = both(c.one_minus_beta2), l2 = both(c.l2), eps = both(-c.eps), decay = both(f.decay);
-  const float2 size = both(-f.step_size), inv = both(f.inv_root_bc2 * c.root_unscale), mz = both(c.minus_zero);
+  const float2 ob2 = both(c.one_minus_beta2), l2 = both(c.l2), mz = both(c.minus_zero);
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
     float2 g = product(g_in[k], scale, mz);
     if (c.l2 != 0.0f) g = add2(g, product(p[k], l2, mz));
     m[k] = add2(product(m[k], b1, mz), product(g, ob1, mz));
     v[k] = add2(product(v[k], b2, mz), product(product(g, g, mz), ob2, mz));
-    float2 nv = mul2(v[k], both(c.root_scale));
-    nv.x = at_least(nv.x, -3.4028234664e38f);
-    nv.y = at_least(nv.y, -3.4028234664e38f);
-    const float2 above_zero = add2(nv, both(-0x1p-126f));
-    const float2 y = make_float2(rsqrt_approx(-above_zero.x), rsqrt_approx(-above_zero.y));
-    float2 nroot = product(nv, y, mz);
-    nroot = fma2(fma2(nroot, nroot, nv), mul2(y, both(0.5f)), nroot);
-    const float2 nd = add2(product(nroot, inv, mz), eps);
-    float2 z = make_float2(rcp_approx(-nd.x), rcp_approx(-nd.y));
-    z = fma2(z, fma2(nd, z, both(1.0f)), z);
-    float2 q = product(m[k], z, mz);
-    q = fma2(fma2(nd, q, m[k]), z, q);
+  }
+}
+
+// The Newton steps make NaN of an infinite operand.  kLarge: one of the lane's second moments may be infinite, or its 2^36-fold where
+// that is what the root is taken of.  The latter are taken as they are then, and an infinite one gives the quotient zero (NaN
+// with an infinite first moment), as dividing by its root does.  Which of the two it is is decided for all of a lane at once, from
+// the largest of its second moments; with 8-bit states from the block's maximum, which the rounding needs anyway.
+template <bool kLarge>
+__device__ __forceinline__ void adamw_apply(float2 (&p)[4], const float2 (&m)[4], const float2 (&v)[4], const AdamWScalars& c,
+                                            const AdamWFactors& f) {
+  const float2 eps = both(-c.eps), decay = both(f.decay), size = both(-f.step_size), mz = both(c.minus_zero);
+  const float2 inv = both(f.inv_root_bc2 * c.root_unscale);
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    float2 q = adamw_quotient(m[k], v[k], c.root_scale, inv, eps, mz);
+    if constexpr (kLarge) {
+      const float infinity = __uint_as_float(0x7f800000u), up = -c.root_scale;
+      const float2 plain = adamw_quotient(m[k], v[k], -1.0f, both(f.inv_root_bc2), eps, mz);
+      if (!(v[k].x * up < infinity)) q.x = v[k].x == infinity ? __fmul_rn(m[k].x, 0.0f) : plain.x;
+      if (!(v[k].y * up < infinity)) q.y = v[k].y == infinity ? __fmul_rn(m[k].y, 0.0f) : plain.y;
+    }
     p[k] = add2(product(p[k], decay, mz), product(q, size, mz));
   }
+}
+
+// Largest of a lane's second moments; NaN where one of them is.
+__device__ __forceinline__ float largest(const float2 (&v)[4]) {
+  return max3_nan(max3_nan(v[0].x, v[0].y, v[1].x), max3_nan(v[1].y, v[2].x, v[2].y), max3_nan(v[3].x, v[3].y, v[3].y));
 }
 
 // The eight elements of a lane: parameters, gradients, moments as they lie in memory.
@@ -532,17 +557,30 @@ struct AdamWRun {
       m.unpack(xm);
       v.unpack(xv);
     }
-    adamw_update(xp, xg, xm, xv, c, f, grad_scale);
-    if constexpr (kRemainder) split_masters(xp, p, r); else p.pack(xp);
+    adamw_moments(xp, xg, xm, xv, c, grad_scale);
     if constexpr (k8) {
+      // One branch for both blocks and for the quotient: a block with a large second moment is a rare one too.
+      using First = Code8<true>;
+      using Second = Code8<false>;
       uint32_t low[8], high[8];
       random_dither<kVec>(key, first, low, high);
-      me = Code8<true>::quantize(xm, low, m);
-      ve = Code8<false>::quantize(xv, high, v);
+      const uint32_t m_top = First::block_top(xm), v_top = Second::block_top(xv);
+      if (!(First::is_rare(m_top) || Second::is_rare(v_top))) {
+        adamw_apply<false>(xp, xm, xv, c, f);
+        me = First::template encode<false>(xm, m_top, low, m);
+        ve = Second::template encode<false>(xv, v_top, high, v);
+      } else {
+        adamw_apply<true>(xp, xm, xv, c, f);
+        me = First::template encode<true>(xm, m_top, low, m);
+        ve = Second::template encode<true>(xv, v_top, high, v);
+      }
     } else {
+      if (largest(xv) * -c.root_scale < __uint_as_float(0x7f800000u)) adamw_apply<false>(xp, xm, xv, c, f);
+      else adamw_apply<true>(xp, xm, xv, c, f);
       m.pack(xm);
       v.pack(xv);
     }
+    if constexpr (kRemainder) split_masters(xp, p, r); else p.pack(xp);
   }
 };
 
@@ -648,9 +686,9 @@ struct AdamWRing {
 // fp32 moments: bound by HBM.  268 M elements: fp32 types 1.13 ms (28 bytes an element, 6.65 TB/s), bf16 gradients 1.06 ms
 // (6.6), bf16 0.91 ms (6.5), bf16 with remainders 1.09 ms (6.4).
 // 8-bit moments: 59 instructions an element for its 10 to 16 bytes.  fp32 types 0.65 ms (6.6 TB/s), bf16 gradients 0.58 ms (6.5),
-// bf16 with remainders 0.64 ms (5.8) and bf16 0.58 ms (4.6): the last is bound by the issue slots (78 % used, the integer
+// bf16 with remainders 0.61 ms (6.1) and bf16 0.54 ms (4.9): the last is bound by the issue slots (78 % used, the integer
 // multiply pipe 73 %).  These are bursts; run without a pause the 8-bit step reaches the GPU's power limit and its clock falls
-// from 1.97 to 1.6 GHz (fp32 types 0.73 ms, bf16 0.59), while the step with fp32 moments does not slow down.
+// from 1.97 to 1.6 GHz (fp32 types 0.70 ms, bf16 0.59), while the step with fp32 moments does not slow down.
 // Three CTAs an SM (80 registers): two are 6 - 12 % slower with bf16 types, four spill.
 template <typename P, typename G, bool kRemainder, bool k8, int kCapacity>
 __global__ void __launch_bounds__(kOptThreads, 3)
@@ -910,7 +948,10 @@ __device__ __forceinline__ uint32_t quantize_run(const Run<T>& run, uint32_t key
 #pragma unroll
     for (int k = 0; k < 8; ++k) low[k] = high[k] = 0x800000u;
   }
-  return Code8<kSigned>::quantize(v, kSigned ? low : high, out);
+  using Code = Code8<kSigned>;
+  const uint32_t top = Code::block_top(v);
+  return Code::is_rare(top) ? Code::template encode<true>(v, top, kSigned ? low : high, out)
+                            : Code::template encode<false>(v, top, kSigned ? low : high, out);
 }
 template <typename T, bool kSigned, bool kRandom>
 __global__ void __launch_bounds__(kOptThreads)

@@ -1,0 +1,119 @@
+"""AdamW, clipping and the block quantiser on the GPU at the ends of their ranges: second moments that overflow, lists made on
+the way, long chunks, unusual layouts and checkpoints that hooks look at."""
+
+import os
+
+import numpy as np
+import pytest
+import torch
+
+from emerging_optimizers_b200 import build as eo_build
+from emerging_optimizers_b200.scalar_optimizers import adamw_step, adamw_step_8bit
+from tests import _scalar_ref as ref
+
+
+pytestmark = pytest.mark.gpu
+
+F32, BF16 = torch.float32, torch.bfloat16
+ULP = 2.0**-24  # one fp32 rounding, relative
+HYPER = dict(lr=3e-3, betas=(0.9, 0.95), eps=1e-8, weight_decay=0.1)
+
+
+@pytest.fixture(scope="module", autouse=True)
+def host_module():
+    if not os.path.exists(eo_build.HOST_OUT):
+        eo_build.build_host()
+
+
+def _randn(n, seed, scale=1.0):
+    return torch.from_numpy((np.random.default_rng(seed).standard_normal(n) * scale).astype(np.float32)).cuda()
+
+
+def _np64(t):
+    return t.detach().cpu().to(torch.float64).numpy()
+
+
+def _same(a, b):
+    """The same bits, NaN included."""
+    width = {1: torch.uint8, 2: torch.int16, 4: torch.int32, 8: torch.int64}[a.element_size()]
+    return a.shape == b.shape and a.dtype == b.dtype and torch.equal(a.view(width), b.view(width))
+
+
+# ---- second moments that overflow ---------------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("eps", [1e-8, 1e-10, 1e-15, 1e-30, 0.0])
+@pytest.mark.parametrize("method", ["decoupled", "l2"])
+def test_second_moments_up_to_infinity(eps, method):
+    """Gradients from 1e-14 to 3e38, in any mix within a lane: over several steps the bits of torch's elementary fp32 operations,
+    for which the quotient by an infinite root is zero.  (0.05 g^2 of the smallest is 2^-98: a root that is rounded to nearest.)"""
+    n = 100_003
+    rng = np.random.default_rng(1)
+    lr, (b1, b2), wd = HYPER["lr"], HYPER["betas"], HYPER["weight_decay"]
+    p, m, v = _randn(n, 2, 0.02), torch.zeros(n, device="cuda"), torch.zeros(n, device="cuda")
+    p0, m0, v0 = p.clone(), m.clone(), v.clone()
+    exponent = rng.uniform(-14, 38.4, n)
+    exponent[: n // 2] = rng.uniform(-8, 8, n // 2)  # whole runs without an overflow beside those that have some
+    for step in (1, 2, 1000):
+        g = rng.choice([-1.0, 1.0], n) * 10.0 ** np.clip(exponent + rng.uniform(-1, 1, n), -14, 38.5)
+        g = torch.from_numpy(g.astype(np.float32)).cuda()
+        adamw_step([p], [g], [m], [v], **{**HYPER, "eps": eps}, step=step, weight_decay_method=method)
+        x = g + p0 * wd if method == "l2" else g
+        p0 = p0 * ref.decay_factor(method, lr, wd)
+        m0 = m0 * b1 + x * (1 - b1)
+        v0 = v0 * b2 + (x * x) * (1 - b2)
+        p0 = p0 - (m0 / (v0.sqrt() * (1 / (1 - b2**step) ** 0.5) + eps)) * (lr / (1 - b1**step))
+        assert _same(m, m0) and _same(v, v0) and _same(p, p0)
+    assert bool(torch.isinf(v).any()) and bool((v > 2.0**92).logical_and(torch.isfinite(v)).any())
+
+
+@pytest.mark.parametrize("kind", ["8-bit", "remainders", "8-bit remainders", "bf16"])
+@pytest.mark.parametrize("eps", [1e-8, 1e-15])
+def test_every_form_takes_an_overflowing_second_moment_alike(kind, eps):
+    """First steps of the other forms: the bits of the fp32 step above (bf16 weights: rounded), and the codes of its moments.
+    Blocks that hold a large first or second moment, or one that is not finite, lie beside blocks that do not."""
+    n = 5001
+    exponent = np.random.default_rng(4).uniform(-14, 37, n)
+    exponent[: n // 2] = np.minimum(exponent[: n // 2], np.repeat([3, 4, 5, 6, 7], 500))  # squares around 2^30
+    g = _randn(n, 3) * torch.from_numpy(10.0**exponent).float().cuda()
+    start = _randn(n, 5, 0.02).bfloat16().float()
+    hyper = {**HYPER, "eps": eps}
+    want, m, v = start.clone(), torch.zeros(n, device="cuda"), torch.zeros(n, device="cuda")
+    adamw_step([want], [g], [m], [v], **hyper, step=1)
+    p = start.clone() if kind == "8-bit" else start.bfloat16()
+    r = [torch.zeros(n, dtype=torch.int16, device="cuda")] if "remainders" in kind else None
+    if "8-bit" in kind:
+        state = [[torch.zeros(k, dtype=torch.uint8, device="cuda")] for k in (n, -(-n // 256), n, -(-n // 256))]
+        adamw_step_8bit([p], [g], *state, **hyper, step=1, seed=0, remainders=r)
+        for ((codes,), (exponents,)), wide, signed in ((state[:2], m, True), (state[2:], v, False)):
+            want_c, want_e = ref.quantize(wide.cpu().numpy(), signed, ref.random_bits(n, 0, 0, 1, signed))
+            assert np.array_equal(codes.cpu().numpy(), want_c) and np.array_equal(exponents.cpu().numpy(), want_e)
+    else:
+        adamw_step([p], [g], *[[torch.zeros(n, device="cuda")] for _ in range(2)], **hyper, step=1, remainders=r)
+    if r is not None:
+        p = torch.from_numpy(ref.join(p.view(torch.int16).cpu().numpy(), r[0].cpu().numpy())).cuda()
+    assert _same(p, want.bfloat16() if kind == "bf16" else want)
+
+
+@pytest.mark.parametrize("size,eps", [(1e15, 1e-15), (1e17, 1e-15), (1e18, 0.0), (1e18, 1e-8)])
+def test_steps_by_large_second_moments_against_float64(size, eps):
+    """Second moments beyond 2^92 that fp32 still holds, with any eps: the first step is about lr."""
+    n = 2000
+    g = _randn(n, 6, size)
+    p, m, v = (torch.zeros(n, device="cuda") for _ in range(3))
+    adamw_step([p], [g], [m], [v], lr=1e-2, betas=(0.9, 0.95), eps=eps, weight_decay=0.0, step=1)
+    m64, v64 = _np64(m), _np64(v)
+    assert np.isfinite(v64).all() and v64.max() > 2.0**92
+    want = -(1e-2 / (1 - 0.9)) * m64 / (np.sqrt(v64 / (1 - 0.95)) + eps)
+    # the root, three products, a sum, the quotient, two factors: at most ten roundings
+    assert np.all(np.abs(_np64(p) - want) <= 15 * ULP * np.abs(want))
+
+
+def test_moments_that_are_not_finite_give_what_their_quotient_is():
+    inf, nan = float("inf"), float("nan")
+    m = torch.tensor([1.0, -1.0, inf, nan, 1.0, 0.0], device="cuda")
+    v = torch.tensor([inf, inf, inf, inf, nan, inf], device="cuda")
+    g, p = torch.zeros(6, device="cuda"), torch.tensor([2.0, 0.0, 2.0, 2.0, 2.0, -0.0], device="cuda")
+    adamw_step([p], [g], [m], [v], **{**HYPER, "weight_decay": 0.0}, step=9)
+    out = p.cpu()
+    assert out[0] == 2 and out[1] == 0 and out[5] == 0 and bool(torch.isnan(out[2:5]).all())
