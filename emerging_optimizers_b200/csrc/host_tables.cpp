@@ -68,15 +68,14 @@ std::string names_of(unsigned types) {
   return s;
 }
 
-// A list or tuple of tensors (borrowed for the lifetime of this object).
+// A list or tuple of tensors, which the caller keeps until its launch: tensors that only an iterator holds would be gone by then.
 class Tensors {
  public:
-  Tensors(PyObject* object, const char* name) : name_(name) {
+  Tensors(PyObject* object, const char* name) : seq_(object), name_(name) {
     if (THPVariable_Check(object)) raise(PyExc_TypeError, name_ + " must be a list of tensors, not a tensor");
-    seq_ = PySequence_Fast(object, "expected a list of tensors");
-    if (seq_ == nullptr) throw Raised{};
+    if (!PyList_Check(object) && !PyTuple_Check(object))
+      raise(PyExc_TypeError, name_ + " must be a list of tensors, not " + Py_TYPE(object)->tp_name);
   }
-  ~Tensors() { Py_XDECREF(seq_); }
   Tensors(const Tensors&) = delete;
   int64_t size() const { return PySequence_Fast_GET_SIZE(seq_); }
   PyObject* item(int64_t i) const { return PySequence_Fast_GET_ITEM(seq_, i); }

@@ -48,6 +48,12 @@ def _device_scalar(value: Any, name: str, device: int, dtype: torch.dtype) -> to
     return value
 
 
+def _listed(tensors: Any) -> Any:
+    """``tensors`` as a list or tuple, which keeps what an iterator or a view makes on the way alive until the launch: the
+    table holds addresses only.  A tensor would be taken apart into its rows: it stays one, and the table refuses it."""
+    return tensors if tensors is None or isinstance(tensors, (list, tuple, torch.Tensor)) else list(tensors)
+
+
 def _step(
     params, grads, m, v, m_exponents, v_exponents, remainders, *, lr, betas, eps, weight_decay, step,
     weight_decay_method, grad_scale, seed=0, first_index=0,
@@ -55,11 +61,14 @@ def _step(
     _check_hyperparameters(lr, betas, eps, weight_decay, weight_decay_method)
     if not (0 <= seed <= _MASK32):
         raise ValueError(f"seed must be in [0, 2^32), got {seed}")
-    if not torch.is_tensor(params):  # a tensor would be taken apart into its rows: the table refuses it
-        params = list(params)
-        if not params:
-            return
+    params, grads, m, v, m_exponents, v_exponents, remainders = map(
+        _listed, (params, grads, m, v, m_exponents, v_exponents, remainders)
+    )
+    if not torch.is_tensor(params) and not params:
+        return
     on_host = isinstance(step, int)
+    if not on_host:
+        step = _listed(step)
     if on_host and step < 1:
         raise ValueError(f"step counts from 1, got {step}")
     host = _native.host()

@@ -117,3 +117,32 @@ def test_moments_that_are_not_finite_give_what_their_quotient_is():
     adamw_step([p], [g], [m], [v], **{**HYPER, "weight_decay": 0.0}, step=9)
     out = p.cpu()
     assert out[0] == 2 and out[1] == 0 and out[5] == 0 and bool(torch.isnan(out[2:5]).all())
+
+
+# ---- lists made on the way ----------------------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_iterators_give_the_bits_of_lists(bits):
+    """Gradients, counters and the rest from generators, with device counters: the scratch that these need is allocated while the
+    tensors made on the way are in use."""
+    sizes = [4, 300, 5000]
+    ps = [_randn(n, i) for i, n in enumerate(sizes)]
+    gs = [_randn(n, 10 + i, 1e-3).bfloat16() for i, n in enumerate(sizes)]
+    outs = []
+    for lazy in (False, True):
+        p = [t.clone() for t in ps]
+        if bits == 32:
+            state = [[torch.zeros_like(t) for t in ps] for _ in range(2)]
+        else:
+            state = [[torch.zeros(k, dtype=torch.uint8, device="cuda") for k in ks] for ks in 2 * (sizes, [-(-n // 256) for n in sizes])]
+        lists = [p, (g.float() for g in gs), *state]
+        step = (torch.full((), 3, device="cuda") for _ in sizes)
+        if lazy:
+            lists = [map(lambda t: t, ts) for ts in lists]
+        else:
+            lists, step = [list(ts) for ts in lists], list(step)
+        call, kw = (adamw_step, {}) if bits == 32 else (adamw_step_8bit, {"seed": 1})
+        call(*lists, **HYPER, **kw, step=step, grad_scale=torch.tensor(0.5, device="cuda"))
+        outs.append([*p, *(t for ts in state for t in ts)])
+    assert all(_same(a, b) for a, b in zip(*outs))

@@ -1,0 +1,62 @@
+"""AdamW, clipping and the block quantiser without a GPU: what a call keeps, and checkpoints and builds that are unusual."""
+
+import gc
+import weakref
+
+import pytest
+import torch
+
+from emerging_optimizers_b200 import _native
+from emerging_optimizers_b200 import build as eo_build
+from emerging_optimizers_b200.scalar_optimizers import adamw_step, adamw_step_8bit
+
+
+@pytest.fixture(scope="module", autouse=True)
+def built():
+    eo_build.build()
+
+
+class _FakeHost:
+    """Stands in for the host module: notes which tensors it was given."""
+
+    def __init__(self):
+        self.seen = []
+
+    def adamw_table(self, *columns):
+        self.seen += [weakref.ref(t) for ts in columns if ts is not None and not torch.is_tensor(ts) for t in ts]
+        return 0, b"", 1
+
+    def stream(self, device):
+        return 0, True, False
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_tensors_made_on_the_way_live_until_the_launch(bits, monkeypatch):
+    """Lists may be iterators that make their tensors as they go: the table holds addresses, so the call has to keep them."""
+    host = _FakeHost()
+    monkeypatch.setattr(_native, "host", lambda: host)
+    alive = []
+
+    def launch(device, n, *args, **kw):
+        gc.collect()
+        assert n == 3
+        alive.extend(r() is not None for r in host.seen)
+
+    monkeypatch.setattr(_native, "adamw_step", launch)
+
+    def made(dtype=torch.float32):
+        return (torch.zeros(4, dtype=dtype) for _ in range(3))
+
+    kw = dict(lr=1e-3, step=(torch.ones((), dtype=torch.int64) for _ in range(3)), remainders=made(torch.int16))
+    if bits == 32:
+        adamw_step(made(), made(), made(), map(torch.abs, made()), **kw)
+    else:
+        adamw_step_8bit(*[made() for _ in range(6)], **kw, seed=0)
+    assert len(alive) == 3 * (6 if bits == 32 else 8) and all(alive)
+
+
+def test_the_table_takes_lists_and_tuples_only():
+    x = torch.zeros(3)
+    for bad in (iter([x]), {0: x}, None, x):
+        with pytest.raises(TypeError, match="must be a list of tensors"):
+            _native.host().grads_table(bad, False)
