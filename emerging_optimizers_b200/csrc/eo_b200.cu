@@ -947,7 +947,7 @@ int eo_adamw_step(int n, const int64_t* host_table, const eo_adamw_config* confi
   if (cfg.decay_method < 0 || cfg.decay_method > 3) return fail(EO_ERR_BAD_ARG, "unknown weight-decay method");
   const int64_t *p = host_table, *g = p + n, *m = g + n, *v = m + n, *me = v + n, *ve = me + n, *r = ve + n, *step = r + n,
                 *numel = step + n, *kind = numel + n;
-  bool device_factors = cfg.dev_lr != nullptr;
+  bool device_factors = cfg.dev_lr != nullptr, config_step = false;
   unsigned kinds = 0;
   for (int i = 0; i < n; ++i) {
     if (numel[i] < 0) return fail(EO_ERR_BAD_ARG, "tensor %d: negative size", i);
@@ -957,9 +957,10 @@ int eo_adamw_step(int n, const int64_t* host_table, const eo_adamw_config* confi
     if (kind[i] < 0 || kind[i] > 7 || ((kind[i] & EO_KIND_REMAINDER) && (!(kind[i] & EO_KIND_PARAM_BF16) || !r[i])))
       return fail(EO_ERR_BAD_ARG, "tensor %d: unknown kind, or remainders without bf16 parameters", i);
     if (step[i]) device_factors = true;
+    else config_step = true;
     kinds |= 1u << kind[i];
   }
-  if (cfg.step < 1 && !device_factors) return fail(EO_ERR_BAD_ARG, "step counts from 1");
+  if (cfg.step < 1 && config_step) return fail(EO_ERR_BAD_ARG, "step counts from 1");
   if (device_factors && (cfg.scratch == nullptr || cfg.scratch_bytes < eo_adamw_scratch_bytes(n)))
     return fail(EO_ERR_WORKSPACE, "adamw scratch: need %zu bytes, got %zu", eo_adamw_scratch_bytes(n), cfg.scratch_bytes);
   eo::AdamWScalars c;

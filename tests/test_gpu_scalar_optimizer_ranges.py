@@ -2,11 +2,13 @@
 the way, long chunks, unusual layouts and checkpoints that hooks look at."""
 
 import os
+import struct
 
 import numpy as np
 import pytest
 import torch
 
+from emerging_optimizers_b200 import _native
 from emerging_optimizers_b200 import build as eo_build
 from emerging_optimizers_b200.scalar_optimizers import adamw_step, adamw_step_8bit
 from tests import _scalar_ref as ref
@@ -146,3 +148,45 @@ def test_iterators_give_the_bits_of_lists(bits):
         call(*lists, **HYPER, **kw, step=step, grad_scale=torch.tensor(0.5, device="cuda"))
         outs.append([*p, *(t for ts in state for t in ts)])
     assert all(_same(a, b) for a, b in zip(*outs))
+
+
+# ---- the C interface ----------------------------------------------------------------------------------------------------
+
+
+def _c_step(counters, *, step, dev_lr=False, eps=1e-8, sizes=(4, 4)):
+    """eo_adamw_step on tensors of ones; counters[i]: whether tensor i has a device step counter."""
+    n = len(sizes)
+    rows = [[torch.ones(k, device="cuda") for k in sizes] for _ in range(4)]
+    count, lr = torch.ones((), dtype=torch.int64, device="cuda"), torch.full((), 0.1, device="cuda")
+    scratch = torch.zeros(_native.lib().eo_adamw_scratch_bytes(n), dtype=torch.uint8, device="cuda")
+    columns = [[t.data_ptr() for t in ts] for ts in rows] + [[0] * n] * 3
+    columns += [[count.data_ptr() if c else 0 for c in counters], list(sizes), [0] * n]
+    table = struct.pack(f"{10 * n}q", *[x for column in columns for x in column])
+    config = _native._CONFIG.pack(
+        0.1, 0.9, 0.95, eps, 0.0, step, lr.data_ptr() if dev_lr else 0, 0, scratch.data_ptr(), scratch.numel(), 0, 32, 0, 0
+    )
+    rc = _native.lib().eo_adamw_step(n, table, config, torch.cuda.current_stream().cuda_stream)
+    torch.cuda.synchronize()
+    return rc, rows[0]
+
+
+BAD_ARG = 1
+
+
+@pytest.mark.parametrize("counters,dev_lr,sizes", [
+    ((0, 0), True, (4, 4)), ((1, 0), False, (4, 4)), ((0, 1), True, (4, 4)), ((0, 0), False, (4, 4)), ((0, 1), False, (4, 0)),
+])  # fmt: skip
+def test_step_numbers_below_one_are_refused_where_a_tensor_uses_them(counters, dev_lr, sizes):
+    for step in (0, -3):
+        rc, params = _c_step(counters, step=step, dev_lr=dev_lr, sizes=sizes)
+        assert rc == BAD_ARG and b"counts from 1" in _native.lib().eo_last_error()
+        assert all(bool((p == 1).all()) for p in params)
+    rc, params = _c_step(counters, step=1, dev_lr=dev_lr, sizes=sizes)
+    assert rc == 0 and all(bool(torch.isfinite(p).all()) and not bool((p == 1).any()) for p in params)
+
+
+@pytest.mark.parametrize("counters,sizes", [((1, 1), (4, 4)), ((1, 0), (4, 0))])
+def test_step_number_is_free_where_every_tensor_has_a_counter(counters, sizes):
+    for dev_lr in (False, True):
+        rc, params = _c_step(counters, step=0, dev_lr=dev_lr, sizes=sizes)
+        assert rc == 0 and all(bool(torch.isfinite(p).all()) for p in params)
