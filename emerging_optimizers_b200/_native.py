@@ -7,11 +7,14 @@ object is missing or a call fails, the functions here raise.
 from __future__ import annotations
 
 import ctypes
+import importlib.util
 import os
 import struct
 from ctypes import POINTER, c_char_p, c_double, c_float, c_int, c_int64, c_size_t, c_uint32, c_void_p
 
 import torch
+
+from emerging_optimizers_b200 import build
 
 
 _LIB_NAME = "libeo_b200.so"
@@ -780,18 +783,19 @@ def host():
     """The module that checks lists of tensors and builds the tables of their addresses (``csrc/host_tables.cpp``)."""
     global _host_module
     if _host_module is None:
+        path = build.host_path()
         try:
-            from emerging_optimizers_b200 import _host
+            if not os.path.exists(path):
+                raise ImportError("there is no such file")
+            spec = importlib.util.spec_from_file_location("emerging_optimizers_b200._host", path)
+            module = importlib.util.module_from_spec(spec)
+            spec.loader.exec_module(module)
         except ImportError as e:
             raise NativeLibraryError(
-                f"the host module cannot be loaded ({e}): build it with `python -m emerging_optimizers_b200.build`"
+                f"no host module that was built for torch {torch.__version__} can be loaded from {path} ({e}): build it "
+                "with `python -m emerging_optimizers_b200.build --force`"
             ) from e
-        if _host.TORCH_VERSION != torch.__version__.split("+")[0]:
-            raise NativeLibraryError(
-                f"the host module was built for torch {_host.TORCH_VERSION}, this is {torch.__version__}: build it "
-                "again with `python -m emerging_optimizers_b200.build --force`"
-            )
-        _host_module = _host
+        _host_module = module
     return _host_module
 
 

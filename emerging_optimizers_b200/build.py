@@ -1,5 +1,5 @@
 """Build ``libeo_b200.so`` in-tree with nvcc for sm_100a (cross-compiles without a GPU), and the Python extension
-``_host.so`` (tables of tensor addresses, ``csrc/host_tables.cpp``) with g++ against the installed torch.
+``_host-torch<version>.<python abi>.so`` (tables of tensor addresses, ``csrc/host_tables.cpp``) with g++ against the installed torch.
 
 Usage: ``python -m emerging_optimizers_b200.build [--force] [--verbose]``
 """
@@ -13,18 +13,28 @@ import subprocess
 import sys
 import sysconfig
 
+import torch
+
 
 PKG_DIR = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(PKG_DIR, "csrc")
 OUT = os.path.join(PKG_DIR, "libeo_b200.so")
 SOURCES = ["eo_b200.cu"]
-HOST_OUT = os.path.join(PKG_DIR, "_host.so")
 HOST_SOURCE = os.path.join(CSRC, "host_tables.cpp")
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
     "-O3", "-std=c++17", "-lineinfo",
     "-shared", "-Xcompiler", "-fPIC",
 ]  # fmt: skip
+
+
+def host_path() -> str:
+    """Path of the host extension for this torch and this Python.  Both are part of its name: a module built against another
+    version has another name, so that it is neither loaded nor taken for up to date."""
+    return os.path.join(PKG_DIR, f"_host-torch{torch.__version__}{sysconfig.get_config_var('EXT_SUFFIX')}")
+
+
+HOST_OUT = host_path()
 
 
 def _nvcc() -> str:
@@ -62,24 +72,24 @@ def _run(cmd: list[str], tmp: str, out: str) -> str:
 
 
 def build_host(force: bool = False) -> str:
-    """Compile the host extension if its source is newer than it; return its path."""
-    if not force and os.path.exists(HOST_OUT) and os.path.getmtime(HOST_SOURCE) <= os.path.getmtime(HOST_OUT):
-        return HOST_OUT
-    import torch
+    """Compile the host extension for this torch and Python if it is missing or its source is newer; return its path."""
+    out = host_path()
+    if not force and os.path.exists(out) and os.path.getmtime(HOST_SOURCE) <= os.path.getmtime(out):
+        return out
     from torch.utils import cpp_extension
 
     cuda_home = os.path.dirname(os.path.dirname(os.path.realpath(_nvcc())))
     includes = [*cpp_extension.include_paths(), os.path.join(cuda_home, "include"), sysconfig.get_paths()["include"]]
     lib_dir = os.path.join(os.path.dirname(torch.__file__), "lib")
-    tmp = f"{HOST_OUT}.{os.getpid()}.tmp"
+    tmp = f"{out}.{os.getpid()}.tmp"
     cmd = [
         shutil.which("g++") or "g++", "-O2", "-std=c++17", "-shared", "-fPIC",
         f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}",
         *[f"-I{p}" for p in includes], "-o", tmp, HOST_SOURCE,
         f"-L{lib_dir}", "-ltorch_python", "-ltorch", "-lc10", "-lc10_cuda", f"-Wl,-rpath,{lib_dir}",
     ]  # fmt: skip
-    _run(cmd, tmp, HOST_OUT)
-    return HOST_OUT
+    _run(cmd, tmp, out)
+    return out
 
 
 def build(force: bool = False, verbose: bool = False, extra_flags: list[str] | None = None) -> str:

@@ -7,7 +7,6 @@
 
 #include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAStream.h>
-#include <torch/version.h>
 
 #include <algorithm>
 #include <cstdint>
@@ -292,10 +291,5 @@ PyModuleDef module = {PyModuleDef_HEAD_INIT, "_host", nullptr, -1, methods, null
 }  // namespace
 
 PyMODINIT_FUNC PyInit__host() {
-  PyObject* m = PyModule_Create(&module);
-  if (m != nullptr && PyModule_AddStringConstant(m, "TORCH_VERSION", TORCH_VERSION) != 0) {
-    Py_DECREF(m);
-    return nullptr;
-  }
-  return m;
+  return PyModule_Create(&module);
 }

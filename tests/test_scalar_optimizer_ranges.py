@@ -1,6 +1,8 @@
 """AdamW, clipping and the block quantiser without a GPU: what a call keeps, and checkpoints and builds that are unusual."""
 
 import gc
+import os
+import shutil
 import weakref
 
 import pytest
@@ -60,3 +62,42 @@ def test_the_table_takes_lists_and_tuples_only():
     for bad in (iter([x]), {0: x}, None, x):
         with pytest.raises(TypeError, match="must be a list of tensors"):
             _native.host().grads_table(bad, False)
+
+
+@pytest.mark.parametrize("version", ["2.11.0a0+git1234567", "2.12.0.dev20260101", "2.11.0a0"])
+def test_host_module_of_a_pre_release_of_torch(version, tmp_path, monkeypatch):
+    """A module built for a pre-release is loaded there, and neither loaded nor taken for up to date with another torch."""
+    real = eo_build.build_host()
+    commands = []
+
+    def compiler(cmd, tmp, out):
+        commands.append(cmd)
+        shutil.copy(real, out)
+        return ""
+
+    monkeypatch.setattr(eo_build, "PKG_DIR", str(tmp_path))
+    monkeypatch.setattr(eo_build, "_run", compiler)
+    monkeypatch.setattr(_native, "_host_module", None)
+    monkeypatch.setattr(torch, "__version__", version)
+    with pytest.raises(_native.NativeLibraryError, match="build --force"):
+        _native.host()
+    path = eo_build.build_host()
+    assert len(commands) == 1 and os.path.dirname(path) == str(tmp_path)
+    assert _native.host().__file__ == path
+    eo_build.build_host()
+    assert len(commands) == 1  # up to date
+    monkeypatch.setattr(_native, "_host_module", None)
+    monkeypatch.setattr(torch, "__version__", "2.11.1")
+    with pytest.raises(_native.NativeLibraryError, match="built for torch 2.11.1"):
+        _native.host()
+    eo_build.build_host()
+    assert len(commands) == 2
+
+
+def test_host_module_that_does_not_load_is_named(tmp_path, monkeypatch):
+    monkeypatch.setattr(eo_build, "PKG_DIR", str(tmp_path))
+    monkeypatch.setattr(_native, "_host_module", None)
+    with open(eo_build.host_path(), "w") as f:
+        f.write("not a module")
+    with pytest.raises(_native.NativeLibraryError, match="build --force"):
+        _native.host()
