@@ -91,8 +91,9 @@ class Tensors {
   std::string name_;
 };
 
-// The checks that every tensor passes, and its address.
-int64_t address(const Tensors& ts, int64_t i, int device, unsigned types, int64_t numel) {
+// The checks that every tensor passes, and its address.  any_order: dense in any order of its dimensions, for operators to which
+// the places of the elements are nothing.
+int64_t address(const Tensors& ts, int64_t i, int device, unsigned types, int64_t numel, bool any_order = false) {
   const at::Tensor& t = ts[i];
   if (!t.is_cuda()) raise_no_cpu_path(ts.at(i), t);
   if (t.get_device() != device)
@@ -102,7 +103,8 @@ int64_t address(const Tensors& ts, int64_t i, int device, unsigned types, int64_
   if (numel >= 0 && t.numel() != numel)
     raise(PyExc_ValueError,
           ts.at(i) + " has " + std::to_string(t.numel()) + " elements where " + std::to_string(numel) + " are needed");
-  if (!t.is_contiguous()) raise(PyExc_ValueError, ts.at(i) + " is not contiguous");
+  if (!t.is_contiguous() && !(any_order && t.is_non_overlapping_and_dense()))
+    raise(PyExc_ValueError, ts.at(i) + (any_order ? " is not dense" : " is not contiguous"));
   if (t.is_neg()) raise(PyExc_ValueError, ts.at(i) + " is a negated view");
   return reinterpret_cast<int64_t>(t.data_ptr());
 }
@@ -226,7 +228,7 @@ PyObject* grads_table(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     unsigned types = 0;
     long long elements = 0;
     for (int64_t i = 0; i < n; ++i) {
-      table[i] = address(g, i, device, kF32 | kBF16, -1);
+      table[i] = address(g, i, device, kF32 | kBF16, -1, true);
       table[n + i] = g[i].numel();
       table[2 * n + i] = g[i].scalar_type() == at::kBFloat16 ? 1 : 0;
       types |= 1u << table[2 * n + i];

@@ -29,8 +29,8 @@ def _norm(grads: Sequence[torch.Tensor], max_norm: float, in_place: bool) -> tor
 
 
 def global_grad_norm(grads: Sequence[torch.Tensor]) -> torch.Tensor:
-    """2-norm of all elements of ``grads`` (contiguous fp32 or bf16 CUDA tensors of one device) as an fp32 scalar
-    tensor.  Squares are summed in float64 in a fixed order: the same call gives the same bits."""
+    """2-norm of all elements of ``grads`` (fp32 or bf16 CUDA tensors of one device, dense in any memory order) as an fp32
+    scalar tensor.  Squares are summed in float64 in a fixed order: the same call gives the same bits."""
     return _norm(grads, math.inf, False)[0]
 
 
@@ -54,6 +54,7 @@ def clip_grad_norm_(
 ) -> torch.Tensor:
     """Clip the global 2-norm of the gradients of ``parameters`` in place, as ``torch.nn.utils.clip_grad_norm_`` does.
 
+    Gradients are dense (channels-last and transposed ones too; no gaps, nothing expanded) and each appears once.
     Parameters without a gradient are passed over; with none left the result is 0.  ``error_if_nonfinite`` raises
     ``RuntimeError`` before anything is scaled if the norm is infinite or NaN (and waits for the device to know).
     """

@@ -10,6 +10,7 @@ import torch
 
 from emerging_optimizers_b200 import _native
 from emerging_optimizers_b200 import build as eo_build
+from emerging_optimizers_b200 import utils
 from emerging_optimizers_b200.scalar_optimizers import adamw_step, adamw_step_8bit
 from tests import _scalar_ref as ref
 
@@ -190,3 +191,49 @@ def test_step_number_is_free_where_every_tensor_has_a_counter(counters, sizes):
     for dev_lr in (False, True):
         rc, params = _c_step(counters, step=0, dev_lr=dev_lr, sizes=sizes)
         assert rc == 0 and all(bool(torch.isfinite(p).all()) for p in params)
+
+
+# ---- clipping of other memory orders --------------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_clipping_of_dense_gradients_in_any_memory_order(dtype):
+    """Transposed and channels-last gradients, with dimensions of one element and an odd offset: the float64 norm, and every element
+    scaled where it lies."""
+    base = _randn(3 + 33 * 70, 1).to(dtype)
+    grads = [
+        base[3:].view(33, 70).t(),
+        _randn(4 * 6 * 5 * 5, 2).to(dtype).reshape(4, 6, 5, 5).to(memory_format=torch.channels_last),
+        _randn(60, 3).to(dtype).reshape(5, 1, 12).transpose(0, 2),
+        _randn(7, 4).to(dtype),
+        torch.empty(3, 0, device="cuda", dtype=dtype).t(),
+    ]
+    assert not any(g.is_contiguous() for g in grads[:3])
+    before = [g.clone() for g in grads]
+    norm = float(np.sqrt(sum((_np64(g) ** 2).sum() for g in grads)))
+    params = [torch.nn.Parameter(torch.zeros_like(g)) for g in grads]
+    for p, g in zip(params, grads):
+        p.grad = g
+    assert abs(float(utils.global_grad_norm(grads)) - norm) <= 2 * ULP * norm
+    assert abs(float(utils.clip_coefficient(grads, 1.0)[1]) * norm - 1) <= 1e-6 / norm + 8 * ULP
+    got = utils.clip_grad_norm_(params, 0.5 * norm)
+    assert abs(float(got) - norm) <= 2 * ULP * norm
+    want = 0.5 * norm / (norm + 1e-6)
+    for p, g, b in zip(params, grads, before):
+        assert p.grad.data_ptr() == g.data_ptr()
+        # the coefficient is at most 6 roundings off, the product one; bf16 results are rounded by 2^-8 at most
+        bound = 8 * ULP + (2.0**-8 * 1.01 if dtype == BF16 else 0)
+        assert np.all(np.abs(_np64(g) - _np64(b) * want) <= bound * np.abs(_np64(b) * want))
+    assert torch.equal(base[:3], _randn(3 + 33 * 70, 1).to(dtype)[:3])  # nothing beside them was scaled
+
+
+def test_gradients_with_gaps_are_refused_by_clipping():
+    x = torch.ones(6, 8, device="cuda")
+    for g in (x[:, ::2], x[:, :4], x[0].expand(5, 8)):
+        p = torch.nn.Parameter(torch.zeros(g.shape, device="cuda"))
+        p.grad = g
+        with pytest.raises(ValueError, match="not dense"):
+            utils.clip_grad_norm_([p], 1e-3)
+        with pytest.raises(ValueError, match="not dense"):
+            utils.clip_coefficient([g], 1e-3)
+    assert bool((x == 1).all())
