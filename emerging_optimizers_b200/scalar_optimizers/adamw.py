@@ -339,17 +339,33 @@ class AdamW(optim.Optimizer):
         Moments of the other width are converted (32 to 8 bits: rounded to nearest); types are kept as this optimizer
         has them, whatever the parameter's.
         """
-        for group in state_dict["param_groups"]:
-            for key in ("amsgrad", "maximize"):
-                if group.get(key):
-                    raise ValueError(f"the saved optimizer ran with {key}, which AdamW does not have")
-        saved = state_dict["state"]
-        super().load_state_dict({**state_dict, "state": {}})
-        ids = [i for group in state_dict["param_groups"] for i in group["params"]]
-        params = [p for group in self.param_groups for p in group["params"]]
-        for i, p in zip(ids, params):
-            if i in saved and saved[i]:
-                self.state[p] = self._loaded_state(p, saved[i])
+        saved: dict[str, Any] = {}
+
+        def take(_: optim.Optimizer, state_dict: dict[str, Any]) -> dict[str, Any]:
+            for group in state_dict["param_groups"]:
+                for key in ("amsgrad", "maximize"):
+                    if group.get(key):
+                        raise ValueError(f"the saved optimizer ran with {key}, which AdamW does not have")
+            saved.update(state_dict)
+            return {**state_dict, "state": {}}  # the base class would cast the state to the parameters' types
+
+        def fill(_: optim.Optimizer) -> None:
+            ids = [i for group in saved["param_groups"] for i in group["params"]]
+            params = [p for group in self.param_groups for p in group["params"]]
+            for i, p in zip(ids, params):
+                if saved["state"].get(i):
+                    self.state[p] = self._loaded_state(p, saved["state"][i])
+
+        # after the last of the optimizer's own hooks on what is loaded, and before the first of those on what has been
+        handles = [
+            self.register_load_state_dict_pre_hook(take),
+            self.register_load_state_dict_post_hook(fill, prepend=True),
+        ]
+        try:
+            super().load_state_dict(state_dict)
+        finally:
+            for handle in handles:
+                handle.remove()
 
     @torch.no_grad()
     def _loaded_state(self, p: torch.Tensor, saved: dict) -> dict:

@@ -10,7 +10,7 @@ import torch
 
 from emerging_optimizers_b200 import _native
 from emerging_optimizers_b200 import build as eo_build
-from emerging_optimizers_b200.scalar_optimizers import adamw_step, adamw_step_8bit
+from emerging_optimizers_b200.scalar_optimizers import AdamW, adamw_step, adamw_step_8bit
 
 
 @pytest.fixture(scope="module", autouse=True)
@@ -101,3 +101,57 @@ def test_host_module_that_does_not_load_is_named(tmp_path, monkeypatch):
         f.write("not a module")
     with pytest.raises(_native.NativeLibraryError, match="build --force"):
         _native.host()
+
+
+def _saved(n=3):
+    """A state of torch's class, as it comes back from a file."""
+    state = {i: {"step": torch.tensor(5.0), "exp_avg": torch.full((n,), 0.5), "exp_avg_sq": torch.full((n,), 2.0)} for i in range(2)}
+    return {"state": state, "param_groups": [{"lr": 0.1, "betas": (0.9, 0.95), "eps": 1e-8, "weight_decay": 0.0, "params": [0, 1]}]}
+
+
+def _params(n=3):
+    return [torch.nn.Parameter(torch.ones(n)) for _ in range(2)]
+
+
+def test_hooks_of_loading_see_and_change_the_state(monkeypatch):
+    monkeypatch.setattr(AdamW, "_loaded_state", lambda self, p, saved: dict(saved))  # what makes GPU tensors of it
+    params = _params()
+    opt = AdamW(params)
+    seen = []
+
+    def renamed(_, state_dict):
+        seen.append(("pre", sorted(state_dict["state"])))
+        return {**state_dict, "state": {0: state_dict["state"][1]}}
+
+    def doubled(_, state_dict):
+        seen.append(("second pre", sorted(state_dict["state"])))
+        state_dict["state"] = {0: {**state_dict["state"][0], "exp_avg": 2 * state_dict["state"][0]["exp_avg"]}}
+
+    opt.register_load_state_dict_pre_hook(doubled)
+    opt.register_load_state_dict_pre_hook(renamed, prepend=True)
+    opt.register_load_state_dict_post_hook(lambda o: seen.append(("post", [p in o.state for p in params])))
+    opt.register_load_state_dict_post_hook(lambda o: seen.append(("first post", [p in o.state for p in params])), prepend=True)
+    saved = _saved()
+    opt.load_state_dict(saved)
+    want = [("pre", [0, 1]), ("second pre", [0]), ("first post", [True, False]), ("post", [True, False])]
+    assert seen == want
+    assert bool((opt.state[params[0]]["exp_avg"] == 1.0).all()) and opt.param_groups[0]["lr"] == 0.1
+    assert sorted(saved["state"]) == [0, 1]  # the caller's is as it was
+    opt.load_state_dict(_saved())  # hooks of one call are gone at the next
+    assert seen == 2 * want
+
+
+def test_a_refused_load_leaves_no_hook_behind(monkeypatch):
+    monkeypatch.setattr(AdamW, "_loaded_state", lambda self, p, saved: dict(saved))
+    opt = AdamW(_params())
+    bad = _saved()
+    bad["param_groups"][0]["amsgrad"] = True
+    with pytest.raises(ValueError, match="amsgrad"):
+        opt.load_state_dict(bad)
+    short = _saved()
+    short["param_groups"][0]["params"] = [0]
+    with pytest.raises(ValueError):
+        opt.load_state_dict(short)
+    assert not opt.state
+    opt.load_state_dict(_saved())
+    assert len(opt.state) == 2
