@@ -225,6 +225,11 @@ class AdamW(optim.Optimizer):
         self.seed = seed
         super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay))
 
+    def __getstate__(self) -> dict[str, Any]:
+        """The base class keeps the groups and the state only; without these nobody could read the state."""
+        own = ("weight_decay_method", "state_bits", "master_remainder", "capturable", "seed")
+        return {**super().__getstate__(), **{name: getattr(self, name) for name in own}}
+
     # -- state -------------------------------------------------------------------------------------------------------
 
     def _has_remainder(self, p: torch.Tensor) -> bool:

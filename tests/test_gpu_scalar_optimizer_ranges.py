@@ -1,6 +1,7 @@
 """AdamW, clipping and the block quantiser on the GPU at the ends of their ranges: second moments that overflow, lists made on
 the way, long chunks, unusual layouts and checkpoints that hooks look at."""
 
+import copy
 import os
 import struct
 
@@ -11,7 +12,7 @@ import torch
 from emerging_optimizers_b200 import _native
 from emerging_optimizers_b200 import build as eo_build
 from emerging_optimizers_b200 import utils
-from emerging_optimizers_b200.scalar_optimizers import adamw_step, adamw_step_8bit
+from emerging_optimizers_b200.scalar_optimizers import AdamW, adamw_step, adamw_step_8bit
 from tests import _scalar_ref as ref
 
 
@@ -237,3 +238,28 @@ def test_gradients_with_gaps_are_refused_by_clipping():
         with pytest.raises(ValueError, match="not dense"):
             utils.clip_coefficient([g], 1e-3)
     assert bool((x == 1).all())
+
+
+# ---- copies and layouts ---------------------------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_a_copied_model_and_optimizer_step_alike(bits, dtype):
+    params = [torch.nn.Parameter(_randn(n, n, 0.02).to(dtype)) for n in (5, 700)]
+    opt = AdamW(params, lr=1e-2, state_bits=bits, master_remainder=True, seed=3, weight_decay_method="independent")
+
+    def step(ps, o, k):
+        for p in ps:
+            p.grad = _randn(p.numel(), 10 * k + p.numel(), 1e-3).to(dtype)
+        o.step()
+
+    step(params, opt, 0)
+    others, other = copy.deepcopy((params, opt))
+    for k in (1, 2):
+        step(params, opt, k)
+        step(others, other, k)
+    for p, q in zip(params, others):
+        assert p is not q and _same(p.detach(), q.detach())
+        for name, value in opt.state[p].items():
+            assert _same(value, other.state[q][name]) if torch.is_tensor(value) else value == other.state[q][name]

@@ -1,7 +1,9 @@
 """AdamW, clipping and the block quantiser without a GPU: what a call keeps, and checkpoints and builds that are unusual."""
 
+import copy
 import gc
 import os
+import pickle
 import shutil
 import weakref
 
@@ -155,3 +157,15 @@ def test_a_refused_load_leaves_no_hook_behind(monkeypatch):
     assert not opt.state
     opt.load_state_dict(_saved())
     assert len(opt.state) == 2
+
+
+@pytest.mark.parametrize("again", [copy.deepcopy, lambda o: pickle.loads(pickle.dumps(o)), copy.copy])
+def test_copies_keep_what_says_how_to_read_the_state(again):
+    kw = dict(weight_decay_method="palm", state_bits=8, master_remainder=True, capturable=True, seed=5)
+    opt = AdamW(_params(), lr=0.25, **kw)
+    other = again(opt)
+    assert {name: getattr(other, name) for name in kw} == kw and other.param_groups[0]["lr"] == 0.25
+    other.step()  # nothing has a gradient
+    other.param_groups[0]["params"][0].grad = torch.ones(3)
+    with pytest.raises(_native.NativeLibraryError, match="no CPU path"):
+        other.step()
