@@ -45,6 +45,8 @@ def _check_hyperparameters(lr: Any, betas: Any, eps: float, weight_decay: float,
 def _device_scalar(value: Any, name: str, device: int, dtype: torch.dtype) -> torch.Tensor:
     if not torch.is_tensor(value) or value.dtype != dtype or value.numel() != 1 or value.get_device() != device:
         raise TypeError(f"{name} must be a {dtype} tensor of one element on cuda:{device}")
+    if value.is_neg():
+        raise ValueError(f"{name} is a negated view")
     return value
 
 

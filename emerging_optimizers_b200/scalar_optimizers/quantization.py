@@ -37,6 +37,8 @@ def quantize_blockwise(
         raise TypeError(f"x must be torch.float32 or torch.bfloat16, got {x.dtype}")
     if not x.is_contiguous():
         raise ValueError(f"x is not contiguous (shape {tuple(x.shape)}, strides {x.stride()})")
+    if x.is_neg():
+        raise ValueError("x is a negated view")
     if seed is not None and not 0 <= seed < 1 << 32:
         raise ValueError(f"seed must be in [0, 2^32), got {seed}")
     codes = torch.empty_like(x, dtype=torch.uint8)

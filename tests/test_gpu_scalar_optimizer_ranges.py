@@ -12,7 +12,7 @@ import torch
 from emerging_optimizers_b200 import _native
 from emerging_optimizers_b200 import build as eo_build
 from emerging_optimizers_b200 import utils
-from emerging_optimizers_b200.scalar_optimizers import AdamW, adamw_step, adamw_step_8bit
+from emerging_optimizers_b200.scalar_optimizers import AdamW, adamw_step, adamw_step_8bit, quantize_blockwise
 from tests import _scalar_ref as ref
 
 
@@ -263,3 +263,17 @@ def test_a_copied_model_and_optimizer_step_alike(bits, dtype):
         assert p is not q and _same(p.detach(), q.detach())
         for name, value in opt.state[p].items():
             assert _same(value, other.state[q][name]) if torch.is_tensor(value) else value == other.state[q][name]
+
+
+def test_negated_views_are_refused():
+    """A lazily negated view (a part of a conjugate) holds its values with the other sign."""
+    x, one = _randn(300, 1), torch.ones((), device="cuda")
+    with pytest.raises(ValueError, match="negated"):
+        quantize_blockwise(torch._neg_view(x), signed=True)
+    lists = [[torch.zeros(4, device="cuda")] for _ in range(4)]
+    for kw in (dict(lr=torch._neg_view(one)), dict(lr=0.1, grad_scale=torch._neg_view(one))):
+        with pytest.raises(ValueError, match="negated"):
+            adamw_step(*lists, **kw, step=1)
+    with pytest.raises(ValueError, match="negated"):
+        adamw_step(*lists, lr=0.1, step=torch._neg_view(torch.ones((), dtype=torch.int64, device="cuda")))
+    assert not any(bool(t.any()) for (t,) in lists)
