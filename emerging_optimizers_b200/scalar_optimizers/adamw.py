@@ -182,6 +182,18 @@ def _flat(t: torch.Tensor, order: tuple[int, ...] | None) -> torch.Tensor:
     return (t if order is None else t.permute(order)).contiguous()
 
 
+def _require_layout(states: Sequence[dict], orders: Sequence[tuple[int, ...] | None]) -> None:
+    """What a step writes must lie as its parameter does: a copy in the parameter's order would take the update with it."""
+    for state, order in zip(states, orders):
+        for name in ("exp_avg", "exp_avg_sq", "remainder"):
+            t = state.get(name)
+            if t is not None and not (t if order is None else t.permute(order)).is_contiguous():
+                raise ValueError(
+                    f"a parameter changed its memory order since its state was made ({name} of shape {tuple(t.shape)} has strides "
+                    f"{t.stride()}): optimizer.load_state_dict(optimizer.state_dict()) lays the state out anew"
+                )
+
+
 @registry.register_optimizer("fused_adamw")
 class AdamW(optim.Optimizer):
     """AdamW whose step takes all tensors of a group in one launch.
@@ -309,6 +321,7 @@ class AdamW(optim.Optimizer):
         contiguous.  Returns their number."""
         if not plain:
             orders = [_memory_order(p) for p in params]
+            _require_layout(states, orders)
             grads = [_flat(g, o) for g, o in zip(grads, orders)]
 
         def column(name):  # type: ignore[no-untyped-def]
@@ -332,6 +345,8 @@ class AdamW(optim.Optimizer):
         except Exception:
             if self.capturable:  # a step that was refused does not count
                 torch._foreach_sub_(step, 1)
+            if plain:
+                _require_layout(states, [None] * len(states))  # says more than that a tensor is not contiguous
             raise
         if not self.capturable:
             for s in states:

@@ -277,3 +277,31 @@ def test_negated_views_are_refused():
     with pytest.raises(ValueError, match="negated"):
         adamw_step(*lists, lr=0.1, step=torch._neg_view(torch.ones((), dtype=torch.int64, device="cuda")))
     assert not any(bool(t.any()) for (t,) in lists)
+
+
+@pytest.mark.parametrize("capturable", [False, True])
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("first,then", [("contiguous_format", "channels_last"), ("channels_last", "contiguous_format")])
+def test_a_parameter_that_changes_its_memory_order(first, then, bits, capturable):
+    """``model.to(memory_format=...)`` between two steps: refused without a trace, and taken once the state is laid out anew."""
+    p = torch.nn.Parameter(_randn(4 * 6 * 5 * 5, 1, 0.02).reshape(4, 6, 5, 5).bfloat16().to(memory_format=getattr(torch, first)))
+    other = torch.nn.Parameter(torch.ones(8, device="cuda"))
+    opt = AdamW([p, other], lr=1e-2, state_bits=bits, master_remainder=True, capturable=capturable)
+    for q in (p, other):
+        q.grad = torch.ones_like(q) * 1e-3
+    opt.step()
+    p.data = p.data.to(memory_format=getattr(torch, then))
+    p.grad = torch.ones_like(p) * 1e-3
+    other.grad = None
+    before = [p.detach().clone(), *(t.clone() for t in opt.state[p].values() if torch.is_tensor(t))]
+    with pytest.raises(ValueError, match="lays the state out anew"):
+        opt.step()
+    after = [p.detach(), *(t for t in opt.state[p].values() if torch.is_tensor(t))]
+    assert all(torch.equal(a, b) for a, b in zip(before, after)) and int(opt.state[p]["step"]) == 1
+    moments, remainder = opt.moments(p), opt.state[p]["remainder"].clone()
+    opt.load_state_dict(opt.state_dict())
+    for x, y in zip(moments, opt.moments(p)):
+        assert torch.equal(x, y)  # one value throughout, so that blocks of another order round to it too
+    assert torch.equal(opt.state[p]["remainder"], remainder)
+    opt.step()
+    assert int(opt.state[p]["step"]) == 2 and not torch.equal(opt.moments(p)[0], moments[0])
