@@ -945,6 +945,8 @@ int eo_adamw_step(int n, const int64_t* host_table, const eo_adamw_config* confi
   const eo_adamw_config& cfg = *config;
   if (cfg.state_bits != 8 && cfg.state_bits != 32) return fail(EO_ERR_BAD_ARG, "state_bits must be 8 or 32");
   if (cfg.decay_method < 0 || cfg.decay_method > 3) return fail(EO_ERR_BAD_ARG, "unknown weight-decay method");
+  // the quotient starts from an approximation of the reciprocal that takes subnormal numbers for zero
+  if (cfg.eps != 0.0 && !(cfg.eps >= 0x1p-126 && cfg.eps < 0x1p126)) return fail(EO_ERR_BAD_ARG, "eps must be 0 or in [2^-126, 2^126)");
   const int64_t *p = host_table, *g = p + n, *m = g + n, *v = m + n, *me = v + n, *ve = me + n, *r = ve + n, *step = r + n,
                 *numel = step + n, *kind = numel + n;
   bool device_factors = cfg.dev_lr != nullptr, config_step = false;

@@ -34,7 +34,7 @@ def _check_hyperparameters(lr: Any, betas: Any, eps: float, weight_decay: float,
         raise ValueError(f"Invalid learning rate: {lr}")
     if not (len(betas) == 2 and all(0.0 <= b < 1.0 for b in betas)):
         raise ValueError(f"Invalid betas: {betas}")
-    if not eps >= 0.0:
+    if eps != 0.0 and not 2.0**-126 <= eps < 2.0**126:  # zero, or a number whose reciprocal is normal in fp32
         raise ValueError(f"Invalid epsilon: {eps}")
     if not weight_decay >= 0.0:
         raise ValueError(f"Invalid weight decay: {weight_decay}")
@@ -119,7 +119,7 @@ def adamw_step(
 
     Args:
         params, grads, exp_avgs, exp_avg_sqs: parameters, gradients, first and second moments, one of each per tensor.
-        lr, betas, eps, weight_decay: as usual; ``lr`` may be an fp32 device scalar.
+        lr, betas, eps, weight_decay: as usual; ``lr`` may be an fp32 device scalar; ``eps`` is zero or from 2^-126 to 2^126.
         step: number of this step, from 1; or int64 device scalars (one for all or one per tensor) holding it, which a
             captured graph reads anew at every replay.
         weight_decay_method: one of :data:`emerging_optimizers_b200.mixin.WeightDecayT`.

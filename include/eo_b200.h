@@ -398,7 +398,7 @@ enum { EO_KIND_PARAM_BF16 = 1, EO_KIND_GRAD_BF16 = 2, EO_KIND_REMAINDER = 4 };
  *   m = beta1 m + (1 - beta1) g,  v = beta2 v + (1 - beta2) g^2,
  *   p = p - (m / (sqrt(v) / sqrt(1 - beta2^t) + eps)) * lr / (1 - beta1^t)
  * with decay = 1 - lr weight_decay (method 0, "decoupled"), 1 - weight_decay (1, "independent"),
- * 1 - lr^2 weight_decay (2, "palm") or 1 (3, "l2").
+ * 1 - lr^2 weight_decay (2, "palm") or 1 (3, "l2").  eps is 0 or in [2^-126, 2^126).
  *
  * host_table: ten rows of n int64 each: addresses of the parameters, gradients, first moments, second moments,
  * exponent bytes of the first and of the second moments (8-bit states, else 0), remainders (or 0), device step counters

@@ -187,6 +187,18 @@ def test_step_numbers_below_one_are_refused_where_a_tensor_uses_them(counters, d
     assert rc == 0 and all(bool(torch.isfinite(p).all()) and not bool((p == 1).any()) for p in params)
 
 
+def test_epsilons_at_the_ends():
+    """A weight that nothing moves stays where it is, down to the smallest eps, and the smallest eps divides; those beyond are refused."""
+    for eps in (2.0**-126, 1e-30, 1e-8, 1e30):
+        p, z = torch.tensor([1.0, -2.0], device="cuda"), torch.zeros(2, device="cuda")
+        m = torch.tensor([0.0, eps], device="cuda")
+        adamw_step([p], [z], [m], [z.clone()], lr=0.25, betas=(0.5, 0.5), eps=eps, weight_decay=0.0, step=1)
+        assert p.tolist() == [1.0, -2.0 - 0.25]  # lr / (1 - 0.5) times half of eps over eps
+    for eps in (1e-40, 2.0**126, float("inf"), float("nan"), -1e-8):
+        rc, params = _c_step((0, 0), step=1, eps=eps)
+        assert rc == BAD_ARG and all(bool((p == 1).all()) for p in params)
+
+
 @pytest.mark.parametrize("counters,sizes", [((1, 1), (4, 4)), ((1, 0), (4, 0))])
 def test_step_number_is_free_where_every_tensor_has_a_counter(counters, sizes):
     for dev_lr in (False, True):

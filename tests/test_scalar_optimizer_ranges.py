@@ -59,6 +59,17 @@ def test_tensors_made_on_the_way_live_until_the_launch(bits, monkeypatch):
     assert len(alive) == 3 * (6 if bits == 32 else 8) and all(alive)
 
 
+@pytest.mark.parametrize("eps", [1e-40, 2.0**-127, 2.0**126, 1e39, float("inf"), float("nan"), -1.0])
+def test_epsilons_without_a_normal_reciprocal_are_refused(eps):
+    with pytest.raises(ValueError, match="epsilon"):
+        AdamW(_params(), eps=eps)
+    x = [torch.zeros(3)]
+    with pytest.raises(ValueError, match="epsilon"):
+        adamw_step(x, x, x, x, lr=0.1, step=1, eps=eps)
+    for fine in (0.0, 2.0**-126, 1e-30, 1.0, 1e30):
+        AdamW(_params(), eps=fine)
+
+
 def test_the_table_takes_lists_and_tuples_only():
     x = torch.zeros(3)
     for bad in (iter([x]), {0: x}, None, x):
