@@ -12,7 +12,13 @@ import torch
 from emerging_optimizers_b200 import _native
 from emerging_optimizers_b200 import build as eo_build
 from emerging_optimizers_b200 import utils
-from emerging_optimizers_b200.scalar_optimizers import AdamW, adamw_step, adamw_step_8bit, quantize_blockwise
+from emerging_optimizers_b200.scalar_optimizers import (
+    AdamW,
+    adamw_step,
+    adamw_step_8bit,
+    dequantize_blockwise,
+    quantize_blockwise,
+)
 from tests import _scalar_ref as ref
 
 
@@ -317,3 +323,39 @@ def test_a_parameter_that_changes_its_memory_order(first, then, bits, capturable
     assert torch.equal(opt.state[p]["remainder"], remainder)
     opt.step()
     assert int(opt.state[p]["step"]) == 2 and not torch.equal(opt.moments(p)[0], moments[0])
+
+
+# ---- long chunks ----------------------------------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("p_dtype,g_dtype", [(BF16, BF16), (F32, BF16)])
+def test_chunks_of_more_runs_than_a_warp_holds_exponents_of(p_dtype, g_dtype):
+    """A warp reads the exponent bytes of 32 of its runs (2048 elements apart) at a time; a launch over more than 320 M elements gives it
+    more.  Random codes and exponents, so that a byte of another run shows: whole chunks against the fp32 step on the decoded
+    moments (weights bit for bit) and the statement of the rounding (codes)."""
+    n = 360_000_000 + 12_345
+    chunk = n // (2048 * 148 * 32) // 4 * 4 * 2048
+    assert chunk > 32 * 2048
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    blocks = -(-n // 256)
+    p = torch.empty(n, dtype=p_dtype, device="cuda").normal_(0, 0.02, generator=gen)
+    g = torch.empty(n, dtype=g_dtype, device="cuda").normal_(0, 1, generator=gen)
+    mc = torch.randint(0, 0x78, (n,), dtype=torch.uint8, device="cuda", generator=gen)  # below the NaN
+    mc += torch.randint(0, 2, (n,), dtype=torch.uint8, device="cuda", generator=gen) * 128
+    vc = torch.randint(0, 0xF8, (n,), dtype=torch.uint8, device="cuda", generator=gen)
+    me, ve = [torch.randint(117, 137, (blocks,), dtype=torch.uint8, device="cuda", generator=gen) for _ in range(2)]
+    parts = []
+    for first in (0, 17 * chunk, n // chunk * chunk - chunk, n // chunk * chunk):
+        here = slice(first, min(first + chunk, n))
+        b = slice(first // 256, -(-here.stop // 256))
+        m = dequantize_blockwise(mc[here].clone(), me[b].clone(), signed=True)
+        v = dequantize_blockwise(vc[here].clone(), ve[b].clone(), signed=False)
+        parts.append((here, b, p[here].clone(), g[here].clone(), m, v))
+    adamw_step_8bit([p], [g], [mc], [me], [vc], [ve], **HYPER, step=6, seed=8)
+    for here, b, p0, g0, m, v in parts:
+        adamw_step([p0], [g0], [m], [v], **HYPER, step=6)
+        assert _same(p[here], p0)
+        for codes, exponents, wide, signed in ((mc, me, m, True), (vc, ve, v, False)):
+            bits = ref.random_bits(wide.numel(), 8, 0, 6, signed, first=here.start)
+            want, want_e = ref.quantize(wide.cpu().numpy(), signed, bits)
+            assert np.array_equal(codes[here].cpu().numpy(), want) and np.array_equal(exponents[b].cpu().numpy(), want_e)
