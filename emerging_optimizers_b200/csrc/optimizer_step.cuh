@@ -618,7 +618,7 @@ struct AdamWCursor {
 };
 
 // Runs of the 8-bit step on their way through shared memory: a warp's own ring of kRingStages runs, filled by asynchronous
-// copies two trips ahead.  Without it the loads wait for the 59 instructions an element that lie between a load and its
+// copies two trips ahead.  Without it the loads wait for the 60 instructions an element that lie between a load and its
 // store, and prefetching into registers costs the occupancy it should replace: 268 M fp32 elements 1028 us without, 650 us
 // with the ring.  Three stages leave room for three CTAs an SM with fp32 types; four (two CTAs) are 4 % slower under a
 // sustained load, two 3 % slower with bf16 gradients.
@@ -684,11 +684,11 @@ struct AdamWRing {
 
 // kRemainder: p is bf16 with remainders.  k8: m and v are codes with exponent bytes.
 // fp32 moments: bound by HBM.  268 M elements: fp32 types 1.13 ms (28 bytes an element, 6.65 TB/s), bf16 gradients 1.06 ms
-// (6.6), bf16 0.91 ms (6.5), bf16 with remainders 1.09 ms (6.4).
-// 8-bit moments: 59 instructions an element for its 10 to 16 bytes.  fp32 types 0.65 ms (6.6 TB/s), bf16 gradients 0.58 ms (6.5),
-// bf16 with remainders 0.61 ms (6.1) and bf16 0.54 ms (4.9): the last is bound by the issue slots (78 % used, the integer
-// multiply pipe 73 %).  These are bursts; run without a pause the 8-bit step reaches the GPU's power limit and its clock falls
-// from 1.97 to 1.6 GHz (fp32 types 0.70 ms, bf16 0.59), while the step with fp32 moments does not slow down.
+// (6.6), bf16 weights 0.98 ms (6.6), both bf16 0.91 ms (6.5), with remainders 1.08 ms (6.4).
+// 8-bit moments: 58 to 60 instructions an element for its 10 to 16 bytes.  fp32 types 0.65 ms (6.6 TB/s), bf16 gradients 0.58 ms (6.5),
+// bf16 weights 0.54 ms (6.0), both bf16 0.54 ms (4.9), with remainders 0.61 ms (6.1): bf16 is bound by the issue slots (79 % used,
+// the pipe of the integer multiplications 74 %).  These are bursts; run without a pause the 8-bit step reaches the GPU's power limit
+// and its clock falls from 1.97 to 1.6 GHz (fp32 types 0.70 ms, bf16 0.59), while the step with fp32 moments does not slow down.
 // Three CTAs an SM (80 registers): two are 6 - 12 % slower with bf16 types, four spill.
 template <typename P, typename G, bool kRemainder, bool k8, int kCapacity>
 __global__ void __launch_bounds__(kOptThreads, 3)
@@ -790,9 +790,10 @@ struct GradEntry {
   uint32_t vec;
 };
 
-// Sum of squares of a lane's eight elements in float64.  Squares of fp32 gradients leave the fp32 range, so fp32 may
-// be used only where they stay well inside it: there pairs of them are added in fp32 (one rounding each) and half the
-// conversions to float64 are saved, which run at an eighth of the rate of the additions and bound the sum of bf16 gradients.
+// Sum of squares of a lane's eight elements.  Squares of fp32 gradients leave the fp32 range, so fp32 may be used only where they
+// stay well inside it: there squares and their sums in pairs are rounded to fp32 (2^-24 of the sum each, so 2^-24 of the norm
+// together) and half the conversions to float64 are saved, which run at an eighth of the rate of the additions and bound the sum
+// of bf16 gradients.
 __device__ __forceinline__ double sum_of_squares(const float2 (&g)[4]) {
   float2 s[4];
 #pragma unroll

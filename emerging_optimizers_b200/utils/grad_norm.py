@@ -30,7 +30,9 @@ def _norm(grads: Sequence[torch.Tensor], max_norm: float, in_place: bool) -> tor
 
 def global_grad_norm(grads: Sequence[torch.Tensor]) -> torch.Tensor:
     """2-norm of all elements of ``grads`` (fp32 or bf16 CUDA tensors of one device, dense in any memory order) as an fp32
-    scalar tensor.  Squares are summed in float64 in a fixed order: the same call gives the same bits."""
+    scalar tensor.  Summed in float64 in a fixed order: the same call gives the same bits.  Squares and their sums in pairs are
+    rounded to fp32 where they stay well inside its range, so that the norm is within two fp32 roundings of the exact
+    one."""
     return _norm(grads, math.inf, False)[0]
 
 

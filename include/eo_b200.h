@@ -432,7 +432,8 @@ int eo_adamw_step(int n, const int64_t* host_table, const eo_adamw_config* confi
 
 /*
  * Global gradient norm of `n` flat dense tensors, fp32 and bf16 mixed as they come.  host_table: three rows of n int64
- * (addresses, element counts, EO_F32 / EO_BF16).  Squares are summed in float64 in a fixed order.
+ * (addresses, element counts, EO_F32 / EO_BF16).  Summed in float64 in a fixed order; squares and their sums in pairs are rounded to
+ * fp32 where they stay well inside its range, so that the norm is within two fp32 roundings of the exact one.
  * out[0] = norm, out[1] = min(1, max_norm / (norm + 1e-6)), fp32, in device memory; NaN stays NaN.
  * in_place: the tensors are multiplied by out[1] afterwards (bf16 rounded to nearest even; untouched when it is 1).
  * `scratch`: eo_grad_norm_scratch_bytes(n, elements of all tensors) bytes, 8-byte aligned.
