@@ -411,8 +411,9 @@ enum { EO_KIND_PARAM_BF16 = 1, EO_KIND_GRAD_BF16 = 2, EO_KIND_REMAINDER = 4 };
  * elements (see eo_quantize_blockwise), rounded at random with bits from (seed, first_index + place in the list, step,
  * element).  Remainders (int16, bf16 parameters only): the fp32 master of a parameter is (bf16 bits << 16) + remainder.
  *
- * `step` counts from 1; it holds for every tensor without a device step counter, with `dev_lr` too.  With `dev_lr` or device step
- * counters the factors that depend on them are computed by a small kernel into `scratch` (eo_adamw_scratch_bytes(n) bytes, 16-byte aligned), so that a captured step can be replayed;
+ * `step` counts from 1; it holds for every tensor without a device step counter, with `dev_lr` too.  With `dev_lr` or device
+ * step counters the factors that depend on them are computed by a small kernel into `scratch` (eo_adamw_scratch_bytes(n)
+ * bytes, 16-byte aligned), so that a captured step can be replayed;
  * the counters are read, not advanced.  `grad_scale`: device fp32 scalar or NULL (1).
  *
  * Stands in for the scalar AdamW updates of emerging_optimizers/scalar_optimizers, one call for a list of parameters.
